@@ -746,6 +746,45 @@ def scatter_kv_blocks(staging, k_cache, v_cache, block_ids):
     ref.scatter_kv_blocks(staging, k_cache, v_cache, block_ids.long())
 
 
+def copy_blocks_(tensors, src, dst, tokens=None) -> None:
+    """t[dst[i]] = t[src[i]] for every tensor t of ``tensors`` and pair i, all
+    in one launch (one for each hundred tensors).
+
+    tensors: contiguous tensors of any types and shapes on one device, their
+    first dimension the blocks of a paged cache or the slots of a state. src,
+    dst: int32 [pairs] on that device. tokens (int32 [pairs]): of paged
+    tensors [blocks, heads, block_size, width] only the first tokens[i] rows
+    of every head are copied, the others stay as they are; below 0 counts as
+    0, above block_size as block_size.
+
+    A pair with an id outside a tensor's blocks (-1, say, as padding) copies
+    nothing there. A block may be the source of many pairs; one that is a
+    destination must be neither a source nor another pair's destination of
+    the same call, or what it ends with is not defined."""
+    tensors = list(tensors)
+    if src.dtype != torch.int32 or dst.dtype != torch.int32 \
+            or (tokens is not None and tokens.dtype != torch.int32):
+        raise ValueError("src, dst and tokens are int32")
+    if src.dim() != 1 or src.shape != dst.shape \
+            or (tokens is not None and tokens.shape != src.shape):
+        raise ValueError("src, dst and tokens hold one value for each pair")
+    for t in tensors:
+        if t.dim() < 1 or not t.is_contiguous():
+            raise ValueError("tensors of blocks are contiguous")
+        if tokens is not None and (t.dim() != 4
+                                   or t.shape[2] != tensors[0].shape[2]):
+            raise ValueError("tokens go with paged tensors [blocks, heads, "
+                             "block_size, width] of one block_size")
+        if t.device != src.device:
+            raise ValueError("tensors and ids are on one device")
+    if src.is_cuda:
+        _require_native()
+        _C.copy_blocks(tensors, src.contiguous(), dst.contiguous(),
+                       None if tokens is None else tokens.contiguous())
+        return
+    ref.copy_blocks(tensors, src, dst, tokens)
+
+
 # ---------------------------------------------------------------- attention
 
 def paged_attention_decode(
@@ -1159,6 +1198,93 @@ def moe_combine_norm(y, pos, w, residual, weight, eps: float):
     out = torch.empty((T, H), dtype=y.dtype, device=y.device)
     return fused_add_rms_norm(moe_combine(out, y, pos, w), residual, weight,
                               eps)
+
+
+# ------------------------------------------------- log-probabilities, beams
+
+MOST_CHOICES = 1024  # of one row or search
+
+
+def _check_rows(logits, k: int, most: int) -> None:
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError("logits are rows of at least one token")
+    if logits.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("logits are float32 or bfloat16")
+    if not 0 <= k <= most:
+        raise ValueError(f"k is {k}, not from 0 to {most}")
+
+
+class TopLogprobs(NamedTuple):
+    """Of every row: the first k log-probabilities (fp32) and their tokens
+    (int32), and the given token's (None where none is given)."""
+    logprobs: torch.Tensor
+    ids: torch.Tensor
+    token_logprobs: Optional[torch.Tensor]
+
+
+def top_logprobs(logits: torch.Tensor, k: int,
+                 token_ids: Optional[torch.Tensor] = None) -> TopLogprobs:
+    """The k largest log-probabilities of every row of logits [R, V], and of
+    the tokens token_ids [R] (int32 or int64), in one pass over the logits.
+
+    logits: fp32 or bf16, rows any number of columns apart. Tokens are
+    ordered by logit, equal ones by token, those at -inf last. A row without a
+    distribution (a NaN or +inf in it, or -inf throughout) is NaN, its tokens
+    0 to k-1. A given token outside [0, V) has -inf. k: 0 to V, at most
+    MOST_CHOICES."""
+    _check_rows(logits, k, min(MOST_CHOICES, logits.shape[-1]))
+    if token_ids is not None:
+        if token_ids.dtype not in (torch.int32, torch.int64) \
+                or token_ids.shape != logits.shape[:1] \
+                or token_ids.device != logits.device:
+            raise ValueError("token_ids are int32 or int64, one for each row, "
+                             "on its device")
+        token_ids = token_ids.contiguous()
+    if logits.is_cuda:
+        _require_native()
+        if logits.stride(1) != 1 and logits.shape[1] > 1:
+            logits = logits.contiguous()
+        return TopLogprobs(*_C.top_logprobs(logits, k, token_ids))
+    return TopLogprobs(*ref.top_logprobs(logits, k, token_ids))
+
+
+class BeamChoice(NamedTuple):
+    """Of every search, best first: cumulative scores (fp32), the beams they
+    continue and the tokens they add (int32)."""
+    scores: torch.Tensor
+    parents: torch.Tensor
+    tokens: torch.Tensor
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor,
+                k: int) -> BeamChoice:
+    """The k best continuations of every search: scores [G, B] (fp32) of its
+    B beams, plus the log-probabilities of logits [G*B, V] (fp32 or bf16, rows
+    any number of columns apart; row g*B + b is beam b of search g).
+
+    Sums are formed in 64 bits and rounded once. Equal ones go by beam, then
+    by logit, then by token. A token at -inf is no continuation, nor is any
+    of a beam whose score is not finite (-inf: a beam that has ended or not
+    begun) or whose row has no distribution (a NaN or +inf in it). Places
+    without a continuation hold score -inf, beam -1 and token -1. k: 1 to
+    MOST_CHOICES; twice the number of beams leaves enough of them where up
+    to one continuation of each beam ends it."""
+    _check_rows(logits, k, MOST_CHOICES)
+    if k < 1:
+        raise ValueError("k is at least 1")
+    if scores.dim() != 2 or scores.dtype != torch.float32 \
+            or scores.device != logits.device:
+        raise ValueError("scores are float32 [searches, beams] on the "
+                         "device of the logits")
+    if scores.numel() != logits.shape[0] or scores.shape[1] < 1:
+        raise ValueError(f"{logits.shape[0]} rows of logits for "
+                         f"{tuple(scores.shape)} beams")
+    if logits.is_cuda:
+        _require_native()
+        if logits.stride(1) != 1 and logits.shape[1] > 1:
+            logits = logits.contiguous()
+        return BeamChoice(*_C.beam_select(logits, scores, k))
+    return BeamChoice(*ref.beam_select(logits, scores, k))
 
 
 compute_cos_sin_cache = ref.compute_cos_sin_cache

@@ -6,8 +6,11 @@
 //    single large RCCL send over an xGMI link (SURVEY.md §2.3 "KV-block
 //    pack/unpack for PD transfer"; §5.8 — pack into large contiguous
 //    sends to hit link peak).
+//  * copy_blocks — blocks of every cache tensor, or slots of every state
+//    tensor, onto others, all tensors in one launch.
 
 #include "common.h"
+#include "logprobs.h"
 
 namespace fi {
 
@@ -139,5 +142,60 @@ template void launch_kv_block_copy<true>(u16*, u16*, u16*, const int*, int,
                                          int64_t, hipStream_t);
 template void launch_kv_block_copy<false>(u16*, u16*, u16*, const int*, int,
                                           int64_t, hipStream_t);
+
+// t[dst] = t[src] of every tensor t and pair, of paged rows only the tokens
+// that are filled. A wave copies one slice of one head of one block. Pairs
+// with an id outside the tensor are passed over.
+__global__ __launch_bounds__(256) void copy_blocks_kernel(
+    const BlockTensors tensors, const int* __restrict__ src,
+    const int* __restrict__ dst, const int* __restrict__ tokens,
+    const int pairs, const int block_size) {
+  const BlockTensor& t = tensors.t[blockIdx.y];
+  const int lane = threadIdx.x % kWaveSize;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
+  const int per = t.heads * t.slices;
+  const int64_t total = static_cast<int64_t>(pairs) * per;
+  for (int64_t u = blockIdx.x * 4ll + wave; u < total; u += gridDim.x * 4ll) {
+    const int p = static_cast<int>(u / per);
+    const int rest = static_cast<int>(u - static_cast<int64_t>(p) * per);
+    const int h = rest / t.slices;
+    const u32 begin = static_cast<u32>(rest - h * t.slices) * kSliceBytes;
+    const int s = src[p], d = dst[p];
+    if (s < 0 || d < 0 || s >= t.blocks || d >= t.blocks) continue;
+    u32 used = t.head_bytes;
+    if (tokens)
+      used = static_cast<u32>(min(max(tokens[p], 0), block_size)) *
+             t.token_bytes;
+    if (begin >= used) continue;
+    const u32 len = min(used - begin, static_cast<u32>(kSliceBytes));
+    const int64_t block_bytes = static_cast<int64_t>(t.heads) * t.head_bytes;
+    const int64_t at = static_cast<int64_t>(h) * t.head_bytes + begin;
+    const char* from = t.data + s * block_bytes + at;
+    char* to = t.data + d * block_bytes + at;
+    if (t.unit == 16) {
+      for (u32 i = lane * 16; i < len; i += kWaveSize * 16)
+        *reinterpret_cast<uint4*>(to + i) =
+            *reinterpret_cast<const uint4*>(from + i);
+    } else if (t.unit == 4) {
+      for (u32 i = lane * 4; i < len; i += kWaveSize * 4)
+        *reinterpret_cast<u32*>(to + i) =
+            *reinterpret_cast<const u32*>(from + i);
+    } else {
+      for (u32 i = lane; i < len; i += kWaveSize) to[i] = from[i];
+    }
+  }
+}
+
+void launch_copy_blocks(const BlockTensors& tensors, int count,
+                        const int* src, const int* dst, const int* tokens,
+                        int pairs, int block_size, hipStream_t stream) {
+  int64_t most = 1;
+  for (int i = 0; i < count; ++i)
+    most = std::max(most, static_cast<int64_t>(pairs) * tensors.t[i].heads *
+                              tensors.t[i].slices);
+  const int grid = static_cast<int>(std::min<int64_t>((most + 3) / 4, 65536));
+  hipLaunchKernelGGL(copy_blocks_kernel, dim3(grid, count), dim3(256), 0,
+                     stream, tensors, src, dst, tokens, pairs, block_size);
+}
 
 }  // namespace fi

@@ -1,0 +1,191 @@
+// PyTorch bindings of the operators that a search with beams runs on:
+// log-probabilities and the choice of beams (logprobs.hip), copies of cache
+// blocks and state slots (cache.hip). Every entry checks its operands against
+// what kernel and grid assume, and runs on the device of its operands, on the
+// current stream there.
+
+#include <torch/extension.h>
+
+#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
+#include <c10/hip/HIPStream.h>
+#include <hip/hip_runtime.h>
+
+#include <tuple>
+#include <vector>
+
+#include "logprobs.h"
+
+namespace {
+
+using fi::u16;
+using Guard = c10::hip::OptionalHIPGuardMasqueradingAsCUDA;
+
+hipStream_t current_stream() {
+  return c10::hip::getCurrentHIPStream().stream();
+}
+
+void check_launch() {
+  const hipError_t e = hipGetLastError();
+  TORCH_CHECK(e == hipSuccess, "launch failed: ", hipGetErrorString(e));
+}
+
+void check_logits(const at::Tensor& t) {
+  TORCH_CHECK(t.is_cuda() && t.dim() == 2 &&
+                  (t.scalar_type() == at::kFloat ||
+                   t.scalar_type() == at::kBFloat16),
+              "logits must be float32 or bfloat16 rows on the GPU");
+  // a grid holds 2^32 threads, some dozen workgroups a row
+  TORCH_CHECK(t.size(1) >= 1 && t.size(1) < (1ll << 30) &&
+                  t.size(0) * t.size(1) / 2048 + t.size(0) < (1ll << 23),
+              "too many logits in one call");
+  TORCH_CHECK(t.stride(1) == 1 || t.size(1) == 1,
+              "the tokens of a row of logits must follow one another");
+}
+
+// scores [G, k], parents [G, k], tokens [G, k]
+std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_select(
+    const at::Tensor& logits, const at::Tensor& scores, int64_t k) {
+  check_logits(logits);
+  TORCH_CHECK(k >= 1 && k <= fi::kMostChoices, "k out of range");
+  TORCH_CHECK(scores.dim() == 2 && scores.scalar_type() == at::kFloat &&
+                  scores.device() == logits.device(),
+              "scores must be float32 [searches, beams] beside the logits");
+  const int64_t G = scores.size(0), B = scores.size(1);
+  TORCH_CHECK(G * B == logits.size(0) && (B >= 1 || G == 0),
+              "one row of logits per beam");
+  const Guard guard(logits.device());
+  const auto f32 = logits.options().dtype(at::kFloat);
+  const auto i32 = logits.options().dtype(at::kInt);
+  at::Tensor s = at::empty({G, k}, f32);
+  at::Tensor p = at::empty({G, k}, i32), t = at::empty({G, k}, i32);
+  if (G == 0) return {s, p, t};
+  const int V = logits.size(1);
+  at::Tensor ws = at::empty({fi::logit_workspace(G * B, V, k)},
+                            logits.options().dtype(at::kByte));
+  const auto run = [&](auto* x) {
+    fi::launch_beam_select(x, logits.stride(0), V, scores.data_ptr<float>(),
+                           scores.stride(0), scores.stride(1), G, B, k,
+                           ws.data_ptr(), s.data_ptr<float>(),
+                           p.data_ptr<int>(), t.data_ptr<int>(),
+                           current_stream());
+  };
+  if (logits.scalar_type() == at::kFloat)
+    run(logits.data_ptr<float>());
+  else
+    run(static_cast<const u16*>(logits.data_ptr()));
+  check_launch();
+  return {s, p, t};
+}
+
+// log-probabilities [R, k], tokens [R, k], of the given tokens [R]
+std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>> top_logprobs(
+    const at::Tensor& logits, int64_t k,
+    const c10::optional<at::Tensor>& given) {
+  check_logits(logits);
+  const int64_t R = logits.size(0);
+  TORCH_CHECK(k >= 0 && k <= fi::kMostChoices && k <= logits.size(1),
+              "k out of range");
+  if (given)
+    TORCH_CHECK(given->device() == logits.device() && given->dim() == 1 &&
+                    given->size(0) == R && given->is_contiguous() &&
+                    (given->scalar_type() == at::kInt ||
+                     given->scalar_type() == at::kLong),
+                "token_ids must be int32 or int64 [rows] beside the logits");
+  const Guard guard(logits.device());
+  const auto f32 = logits.options().dtype(at::kFloat);
+  at::Tensor lp = at::empty({R, k}, f32);
+  at::Tensor ids = at::empty({R, k}, logits.options().dtype(at::kInt));
+  c10::optional<at::Tensor> of;
+  if (given) of = at::empty({R}, f32);
+  if (R == 0 || (k == 0 && !given)) return {lp, ids, of};
+  const int V = logits.size(1);
+  at::Tensor ws = at::empty({fi::logit_workspace(R, V, k)},
+                            logits.options().dtype(at::kByte));
+  const bool wide = given && given->scalar_type() == at::kLong;
+  const auto run = [&](auto* x) {
+    fi::launch_top_logprobs(x, logits.stride(0), R, V, k,
+                            given ? given->data_ptr() : nullptr, wide,
+                            ws.data_ptr(), lp.data_ptr<float>(),
+                            ids.data_ptr<int>(),
+                            of ? of->data_ptr<float>() : nullptr,
+                            current_stream());
+  };
+  if (logits.scalar_type() == at::kFloat)
+    run(logits.data_ptr<float>());
+  else
+    run(static_cast<const u16*>(logits.data_ptr()));
+  check_launch();
+  return {lp, ids, of};
+}
+
+void copy_blocks(const std::vector<at::Tensor>& tensors, const at::Tensor& src,
+                 const at::Tensor& dst,
+                 const c10::optional<at::Tensor>& tokens) {
+  TORCH_CHECK(src.is_cuda() && src.scalar_type() == at::kInt &&
+                  src.dim() == 1 && src.is_contiguous(),
+              "src must be int32 ids on the GPU");
+  const int64_t pairs = src.numel();
+  const auto ids = [&](const at::Tensor& t, const char* what) {
+    TORCH_CHECK(t.device() == src.device() && t.scalar_type() == at::kInt &&
+                    t.dim() == 1 && t.is_contiguous() && t.numel() == pairs,
+                what, " must be int32, one for each of src, beside it");
+  };
+  ids(dst, "dst");
+  if (tokens) ids(*tokens, "tokens");
+  TORCH_CHECK(pairs < (1ll << 31), "too many pairs");
+  int block_size = -1;
+  for (const auto& t : tensors) {
+    TORCH_CHECK(t.device() == src.device() && t.dim() >= 1 &&
+                    t.is_contiguous(),
+                "tensors of blocks must be contiguous and beside src");
+    if (!tokens) continue;
+    TORCH_CHECK(t.dim() == 4,
+                "tokens go with paged tensors [blocks, heads, tokens, width]");
+    TORCH_CHECK(block_size < 0 || t.size(2) == block_size,
+                "paged tensors of one call have blocks of one size");
+    TORCH_CHECK(t.size(2) < (1ll << 31), "too many tokens in a block");
+    block_size = static_cast<int>(t.size(2));
+  }
+  if (pairs == 0) return;
+  const Guard guard(src.device());
+  fi::BlockTensors table;
+  int count = 0;
+  const auto flush = [&] {
+    if (count == 0) return;
+    fi::launch_copy_blocks(table, count, src.data_ptr<int>(),
+                           dst.data_ptr<int>(),
+                           tokens ? tokens->data_ptr<int>() : nullptr, pairs,
+                           block_size, current_stream());
+    check_launch();
+    count = 0;
+  };
+  for (const auto& t : tensors) {
+    if (t.numel() == 0) continue;
+    const int64_t block = t.numel() / t.size(0) * t.element_size();
+    const int64_t heads = tokens ? t.size(1) : 1;
+    const int64_t token = tokens ? t.size(3) * t.element_size() : block;
+    TORCH_CHECK(block < (1ll << 31) && t.size(0) < (1ll << 31),
+                "a block must be smaller than 2 GiB");
+    const auto bits =
+        reinterpret_cast<uintptr_t>(t.data_ptr()) | block | token;
+    fi::BlockTensor& e = table.t[count++];
+    e.data = static_cast<char*>(t.data_ptr());
+    e.head_bytes = static_cast<fi::u32>(block / heads);
+    e.token_bytes = static_cast<fi::u32>(token);
+    e.heads = static_cast<int>(heads);
+    e.slices = static_cast<int>((block / heads + fi::kSliceBytes - 1) /
+                                fi::kSliceBytes);
+    e.blocks = static_cast<int>(t.size(0));
+    e.unit = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
+    if (count == fi::kBlockTensors) flush();
+  }
+  flush();
+}
+
+}  // namespace
+
+void register_search_ops(pybind11::module& m) {
+  m.def("beam_select", &beam_select, "the k best continuations of every search");
+  m.def("top_logprobs", &top_logprobs, "top and given log-probabilities");
+  m.def("copy_blocks", &copy_blocks, "blocks of tensors onto others");
+}

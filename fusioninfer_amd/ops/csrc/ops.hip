@@ -850,7 +850,11 @@ void many_rows_gemm_fp8(at::Tensor out, at::Tensor x, at::Tensor x_scales,
 
 }  // namespace
 
+// bindings of a unit of their own (logprobs_bindings.hip)
+void register_search_ops(pybind11::module& m);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  register_search_ops(m);
   m.def("rms_norm", &rms_norm, "RMSNorm (bf16, fp32 accum)");
   m.def("stream_norm", &stream_norm, "RMSNorm (fp32 to bf16)");
   m.def("fused_add_rms_norm", &fused_add_rms_norm,

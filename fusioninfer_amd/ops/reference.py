@@ -425,3 +425,68 @@ def moe_route(logits, k: int, score: str, renorm: bool, scale: float):
     if renorm:
         topv = topv / (topv.sum(dim=-1, keepdim=True) + 1e-20)
     return topv * scale, topi.int()
+
+
+def _first_of(values: torch.Tensor, k: int) -> torch.Tensor:
+    """Indices of the k largest of one row, equal ones by index."""
+    least = values.topk(k).values[-1]
+    at = torch.nonzero(values >= least).view(-1)
+    order = torch.sort(values[at], descending=True, stable=True).indices
+    return at[order[:k]]
+
+
+def top_logprobs(logits, k: int, token_ids=None):
+    """fp32 log_softmax; a row without a distribution is NaN throughout and
+    lists its first k tokens."""
+    lp = torch.log_softmax(logits.float(), dim=-1)
+    R, V = lp.shape
+    ids = torch.arange(k, dtype=torch.int32).repeat(R, 1)
+    for r in range(R):
+        if k and not torch.isnan(lp[r]).any():
+            ids[r] = _first_of(logits[r].float(), k)
+    top = torch.gather(lp, 1, ids.long())
+    if token_ids is None:
+        return top, ids, None
+    at = token_ids.long()
+    inside = (at >= 0) & (at < V)
+    given = torch.gather(lp, 1, at.clamp(0, V - 1).view(-1, 1)).view(-1)
+    given = torch.where(inside | torch.isnan(given), given,
+                        torch.full_like(given, float("-inf")))
+    return top, ids, given
+
+
+def beam_select(logits, scores, k: int):
+    """Scores in 64 bits; equal ones by beam, then by logit, then by token."""
+    G, B = scores.shape
+    V = logits.shape[1]
+    x = logits.double()
+    lp = torch.log_softmax(x, dim=-1).view(G, B, V)
+    total = scores.double().unsqueeze(-1) + lp
+    usable = torch.isfinite(total) & torch.isfinite(scores).unsqueeze(-1)
+    out = torch.full((G, k), float("-inf"), dtype=torch.float32)
+    parents = torch.full((G, k), -1, dtype=torch.int32)
+    tokens = torch.full((G, k), -1, dtype=torch.int32)
+    for g in range(G):
+        b, t = torch.nonzero(usable[g], as_tuple=True)
+        order = torch.sort(x[g * B + b, t], descending=True,
+                           stable=True).indices
+        order = order[torch.sort(b[order], stable=True).indices]
+        b, t = b[order], t[order]
+        s, order = torch.sort(total[g, b, t], descending=True, stable=True)
+        n = min(k, len(s))
+        out[g, :n] = s[:n].float()
+        parents[g, :n] = b[order[:n]].int()
+        tokens[g, :n] = t[order[:n]].int()
+    return out, parents, tokens
+
+
+def copy_blocks(tensors, src, dst, tokens=None) -> None:
+    for t in tensors:
+        for i, (a, b) in enumerate(zip(src.tolist(), dst.tolist())):
+            if not (0 <= a < len(t) and 0 <= b < len(t)):
+                continue
+            if tokens is None:
+                t[b] = t[a]
+            else:
+                n = min(max(int(tokens[i]), 0), t.shape[2])
+                t[b, :, :n] = t[a, :, :n]
