@@ -1203,6 +1203,7 @@ def moe_combine_norm(y, pos, w, residual, weight, eps: float):
 # ------------------------------------------------- log-probabilities, beams
 
 MOST_CHOICES = 1024  # of one row or search
+MOST_BEAMS = 1024    # of one search
 
 
 def _check_rows(logits, k: int, most: int) -> None:
@@ -1266,8 +1267,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor,
     by logit, then by token. A token at -inf is no continuation, nor is any
     of a beam whose score is not finite (-inf: a beam that has ended or not
     begun) or whose row has no distribution (a NaN or +inf in it). Places
-    without a continuation hold score -inf, beam -1 and token -1. k: 1 to
-    MOST_CHOICES; twice the number of beams leaves enough of them where up
+    without a continuation hold score -inf, beam -1 and token -1. B: up to
+    MOST_BEAMS. k: 1 to MOST_CHOICES; twice the number of beams leaves enough of them where up
     to one continuation of each beam ends it."""
     _check_rows(logits, k, MOST_CHOICES)
     if k < 1:
@@ -1276,7 +1277,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor,
             or scores.device != logits.device:
         raise ValueError("scores are float32 [searches, beams] on the "
                          "device of the logits")
-    if scores.numel() != logits.shape[0] or scores.shape[1] < 1:
+    if scores.numel() != logits.shape[0] \
+            or not 1 <= scores.shape[1] <= MOST_BEAMS:
         raise ValueError(f"{logits.shape[0]} rows of logits for "
                          f"{tuple(scores.shape)} beams")
     if logits.is_cuda:

@@ -7,9 +7,10 @@
 namespace fi {
 
 constexpr int kMostChoices = 1024;
+constexpr int kMostBeams = 1024;  // of one search
 
-// bytes of workspace of a call on R rows of V tokens
-int64_t logit_workspace(int64_t R, int V, int k);
+// bytes of workspace of a call on R rows of V tokens of `size` bytes
+int64_t logit_workspace(int64_t R, int V, int k, int size);
 
 template <typename A>
 void launch_beam_select(const A* logits, int64_t stride, int V,

@@ -51,8 +51,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_select(
                   scores.device() == logits.device(),
               "scores must be float32 [searches, beams] beside the logits");
   const int64_t G = scores.size(0), B = scores.size(1);
-  TORCH_CHECK(G * B == logits.size(0) && (B >= 1 || G == 0),
+  TORCH_CHECK(G * B == logits.size(0) && (B >= 1 || G == 0) &&
+                  B <= fi::kMostBeams,
               "one row of logits per beam");
+  // choices of a search are counted in 32 bits
+  TORCH_CHECK((logits.size(1) / 1024 + 2) * B * k < (1ll << 31),
+              "too many logits and choices in one search");
   const Guard guard(logits.device());
   const auto f32 = logits.options().dtype(at::kFloat);
   const auto i32 = logits.options().dtype(at::kInt);
@@ -60,7 +64,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_select(
   at::Tensor p = at::empty({G, k}, i32), t = at::empty({G, k}, i32);
   if (G == 0) return {s, p, t};
   const int V = logits.size(1);
-  at::Tensor ws = at::empty({fi::logit_workspace(G * B, V, k)},
+  at::Tensor ws = at::empty({fi::logit_workspace(G * B, V, std::min<int64_t>(k, V),
+                                                 logits.element_size())},
                             logits.options().dtype(at::kByte));
   const auto run = [&](auto* x) {
     fi::launch_beam_select(x, logits.stride(0), V, scores.data_ptr<float>(),
@@ -99,7 +104,7 @@ std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>> top_logprobs(
   if (given) of = at::empty({R}, f32);
   if (R == 0 || (k == 0 && !given)) return {lp, ids, of};
   const int V = logits.size(1);
-  at::Tensor ws = at::empty({fi::logit_workspace(R, V, k)},
+  at::Tensor ws = at::empty({fi::logit_workspace(R, V, k, logits.element_size())},
                             logits.options().dtype(at::kByte));
   const bool wide = given && given->scalar_type() == at::kLong;
   const auto run = [&](auto* x) {

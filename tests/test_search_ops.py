@@ -215,6 +215,9 @@ def test_refusals(device):
         lambda: ops.beam_select(x, c.double(), 2),
         lambda: ops.beam_select(x, c.view(-1), 2),
         lambda: ops.beam_select(x[:0], c[:, :0], 2),
+        lambda: ops.beam_select(
+            x.new_zeros(ops.MOST_BEAMS + 1, 3),
+            x.new_zeros(1, ops.MOST_BEAMS + 1), 2),
         lambda: ops.top_logprobs(x, 11),
         lambda: ops.top_logprobs(x, -1),
         lambda: ops.top_logprobs(x.double(), 2),
