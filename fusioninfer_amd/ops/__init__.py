@@ -762,6 +762,10 @@ def copy_blocks_(tensors, src, dst, tokens=None) -> None:
     destination must be neither a source nor another pair's destination of
     the same call, or what it ends with is not defined."""
     tensors = list(tensors)
+    if src.is_cuda:
+        _require_native()
+        _C.copy_blocks(tensors, src, dst, tokens)
+        return
     if src.dtype != torch.int32 or dst.dtype != torch.int32 \
             or (tokens is not None and tokens.dtype != torch.int32):
         raise ValueError("src, dst and tokens are int32")
@@ -771,17 +775,12 @@ def copy_blocks_(tensors, src, dst, tokens=None) -> None:
     for t in tensors:
         if t.dim() < 1 or not t.is_contiguous():
             raise ValueError("tensors of blocks are contiguous")
+        if t.device != src.device:
+            raise ValueError("tensors and ids are on one device")
         if tokens is not None and (t.dim() != 4
                                    or t.shape[2] != tensors[0].shape[2]):
             raise ValueError("tokens go with paged tensors [blocks, heads, "
                              "block_size, width] of one block_size")
-        if t.device != src.device:
-            raise ValueError("tensors and ids are on one device")
-    if src.is_cuda:
-        _require_native()
-        _C.copy_blocks(tensors, src.contiguous(), dst.contiguous(),
-                       None if tokens is None else tokens.contiguous())
-        return
     ref.copy_blocks(tensors, src, dst, tokens)
 
 
@@ -1202,8 +1201,8 @@ def moe_combine_norm(y, pos, w, residual, weight, eps: float):
 
 # ------------------------------------------------- log-probabilities, beams
 
-MOST_CHOICES = 1024  # of one row or search
-MOST_BEAMS = 1024    # of one search
+MOST_CHOICES = 256  # of one row or search
+MOST_BEAMS = 256    # of one search
 
 
 def _check_rows(logits, k: int, most: int) -> None:
@@ -1233,19 +1232,16 @@ def top_logprobs(logits: torch.Tensor, k: int,
     distribution (a NaN or +inf in it, or -inf throughout) is NaN, its tokens
     0 to k-1. A given token outside [0, V) has -inf. k: 0 to V, at most
     MOST_CHOICES."""
-    _check_rows(logits, k, min(MOST_CHOICES, logits.shape[-1]))
-    if token_ids is not None:
-        if token_ids.dtype not in (torch.int32, torch.int64) \
-                or token_ids.shape != logits.shape[:1] \
-                or token_ids.device != logits.device:
-            raise ValueError("token_ids are int32 or int64, one for each row, "
-                             "on its device")
-        token_ids = token_ids.contiguous()
     if logits.is_cuda:
         _require_native()
-        if logits.stride(1) != 1 and logits.shape[1] > 1:
-            logits = logits.contiguous()
         return TopLogprobs(*_C.top_logprobs(logits, k, token_ids))
+    _check_rows(logits, k, min(MOST_CHOICES, logits.shape[-1]))
+    if token_ids is not None \
+            and (token_ids.dtype not in (torch.int32, torch.int64)
+                 or token_ids.shape != logits.shape[:1]
+                 or token_ids.device != logits.device):
+        raise ValueError("token_ids are int32 or int64, one for each row, "
+                         "on its device")
     return TopLogprobs(*ref.top_logprobs(logits, k, token_ids))
 
 
@@ -1270,6 +1266,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor,
     without a continuation hold score -inf, beam -1 and token -1. B: up to
     MOST_BEAMS. k: 1 to MOST_CHOICES; twice the number of beams leaves enough of them where up
     to one continuation of each beam ends it."""
+    if logits.is_cuda:
+        _require_native()
+        return BeamChoice(*_C.beam_select(logits, scores, k))
     _check_rows(logits, k, MOST_CHOICES)
     if k < 1:
         raise ValueError("k is at least 1")
@@ -1281,11 +1280,6 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor,
             or not 1 <= scores.shape[1] <= MOST_BEAMS:
         raise ValueError(f"{logits.shape[0]} rows of logits for "
                          f"{tuple(scores.shape)} beams")
-    if logits.is_cuda:
-        _require_native()
-        if logits.stride(1) != 1 and logits.shape[1] > 1:
-            logits = logits.contiguous()
-        return BeamChoice(*_C.beam_select(logits, scores, k))
     return BeamChoice(*ref.beam_select(logits, scores, k))
 
 

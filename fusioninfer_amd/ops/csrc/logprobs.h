@@ -6,8 +6,8 @@
 
 namespace fi {
 
-constexpr int kMostChoices = 1024;
-constexpr int kMostBeams = 1024;  // of one search
+constexpr int kMostChoices = 256;
+constexpr int kMostBeams = 256;  // of one search
 
 // bytes of workspace of a call on R rows of V tokens of `size` bytes
 int64_t logit_workspace(int64_t R, int V, int k, int size);

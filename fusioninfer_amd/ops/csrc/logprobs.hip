@@ -11,12 +11,10 @@
 // a row in registers, and finds its maximum, its sum and its first k keys. The
 // second joins the chunks of a row, or of all rows of a search.
 //
-// First k of what the threads of a workgroup hold: the threads form at least k
-// groups; the least of the groups' maxima is a bound that k values or more
-// reach, and few more (of random values about k ln k, 54 of 16384 at k = 16).
-// Those are written to LDS, and each one's rank among them is its place. Where
-// too many values reach the bound (equal ones, or masked ones that leave a
-// group without any), the k are found in as many rounds of a maximum instead.
+// First k of what a workgroup holds: of the maxima of separate groups of values
+// the k-th largest is a bound that k values or more reach, and few more (18 of
+// 16384 random ones at k = 16 and 64 groups). Those are written to LDS, and each
+// one's rank among them is its place.
 
 #include <hip/hip_runtime.h>
 
@@ -66,8 +64,9 @@ FI_DEV int token_of(u64 key) {
   return static_cast<int>(0xffffffffu - static_cast<u32>(key));
 }
 
-// The partner's value for a step of a reduction that has made all lanes of
-// the step's halves equal: 1, 2, 4, 8, 16 or 32 lanes away.
+// The value of the lane 32, 16, 8, 4, 2 or 1 away, in a reduction that goes
+// through these steps in turn: 4 away by a rotation, which takes what repeats
+// every 8 lanes.
 template <int STEP>
 FI_DEV u32 partner(u32 v) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -75,12 +74,11 @@ FI_DEV u32 partner(u32 v) {
     const auto r = STEP == 32
                        ? __builtin_amdgcn_permlane32_swap(v, v, false, false)
                        : __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    const int lane = __lane_id();
-    return lane & STEP ? r[0] : r[1];
+    return __lane_id() & STEP ? r[0] : r[1];
   } else {
-    // quad_perm [1,0,3,2] and [2,3,0,1], row_half_mirror, row_mirror
+    // row_ror:8, row_ror:4, quad_perm [2,3,0,1] and [1,0,3,2]
     constexpr int ctrl =
-        STEP == 1 ? 0xB1 : STEP == 2 ? 0x4E : STEP == 4 ? 0x141 : 0x140;
+        STEP == 8 ? 0x128 : STEP == 4 ? 0x124 : STEP == 2 ? 0x4E : 0xB1;
     return __builtin_amdgcn_update_dpp(0, v, ctrl, 0xF, 0xF, true);
   }
 #else
@@ -102,36 +100,22 @@ FI_DEV double partner(double v) {
       partner<STEP>(static_cast<u64>(__double_as_longlong(v))));
 }
 
-// v of the lane's group of `lanes` lanes (a power of two), and of the wave
+// over the wave, in every lane
 template <class T, class Op>
-FI_DEV T over_group(T v, int lanes, Op op) {
-  if (lanes > 1) v = op(v, partner<1>(v));
-  if (lanes > 2) v = op(v, partner<2>(v));
-  if (lanes > 4) v = op(v, partner<4>(v));
-  if (lanes > 8) v = op(v, partner<8>(v));
-  if (lanes > 16) v = op(v, partner<16>(v));
-  if (lanes > 32) v = op(v, partner<32>(v));
-  return v;
+FI_DEV T over_wave(T v, Op op) {
+  v = op(v, partner<32>(v));
+  v = op(v, partner<16>(v));
+  v = op(v, partner<8>(v));
+  v = op(v, partner<4>(v));
+  v = op(v, partner<2>(v));
+  return op(v, partner<1>(v));
 }
 template <class T>
 FI_DEV T larger(T a, T b) {
   return a > b ? a : b;
 }
-template <class T>
-FI_DEV T smaller(T a, T b) {
-  return a < b ? a : b;
-}
-template <class T>
-FI_DEV T wave_max(T v) {
-  return over_group(v, kWaveSize, larger<T>);
-}
-
-// lanes of a group so that 64 * WAVES threads form at least k of them
-template <int WAVES>
-FI_DEV int group_lanes(int k) {
-  int lanes = kWaveSize;
-  while (lanes > 1 && WAVES * kWaveSize / lanes < k) lanes >>= 1;
-  return lanes;
+FI_DEV double wave_sum(double v) {
+  return over_wave(v, [](double a, double b) { return a + b; });
 }
 
 // Sum of a chunk and its maximum.
@@ -142,6 +126,24 @@ struct alignas(16) ChunkSum {
 
 constexpr int kHeld = 320;  // of a wave, in LDS
 
+// The order of the k-th largest of the wave's N * 64 values, from its upper
+// bits down to bit LAST; the others are 0.
+template <int LAST, int N>
+FI_DEV u32 reached_by(const float (&v)[N], int k) {
+  u32 order[N], bound = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) order[i] = order_of(v[i]);
+#pragma unroll
+  for (int bit = 31; bit >= LAST; --bit) {
+    const u32 next = bound | 1u << bit;
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) count += __popcll(__ballot(order[i] >= next));
+    if (count >= k) bound = next;
+  }
+  return bound;
+}
+
 // A workgroup's chunk: VC groups of the logits that 16 bytes hold, NV of them a
 // thread. They are counted from the row's first logit wherever it lies, so that
 // equal rows have equal sums; what the last group lacks counts as -inf.
@@ -149,19 +151,21 @@ constexpr int kHeld = 320;  // of a wave, in LDS
 // Four instructions per logit and the exponential's four cycles more are about
 // what memory leaves time for, so everything else is done per piece or per
 // thread: sums go on in 64 bits every piece (a sum that one term dominates
-// keeps the others), and the bound is found from the threads' maxima.
+// keeps the others), the bound is found from the threads' maxima, and the
+// logits of a piece are looked at only where its maximum reaches it.
 template <typename A, int NV>
 __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
     const A* __restrict__ logits, const int64_t stride, const int V,
-    const int chunks, const int VC, const int k, ChunkSum* __restrict__ sums,
-    u64* __restrict__ keys) {
+    const int chunks, const int VC, const int B, const int k,
+    ChunkSum* __restrict__ sums, u64* __restrict__ keys) {
   constexpr int L = kLanes<A>;
-  __shared__ float s_max[kWaves], s_bound[kWaves];
+  __shared__ float s_max[kThreads];
   __shared__ double s_sum[kWaves];
   __shared__ int s_count[kWaves];
   __shared__ u64 s_key[kWaves][kHeld];
   const int tid = threadIdx.x, lane = tid % kWaveSize;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWaveSize);
+  const u64 below = (1ull << lane) - 1;
   const int64_t r = blockIdx.x / chunks;
   const int c = static_cast<int>(blockIdx.x - r * chunks);
   const A* row = logits + r * stride;
@@ -196,62 +200,66 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
     }
   }
 
-  float x[L], m = -INFINITY;
+  float x[L], piece[NV], m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     unpack(raw[i], x, row);
+    piece[i] = x[0];
 #pragma unroll
-    for (int e = 0; e < L; ++e) m = fmaxf(m, x[e]);
+    for (int e = 1; e < L; ++e) piece[i] = fmaxf(piece[i], x[e]);
+    m = fmaxf(m, piece[i]);
   }
-  const int lanes = group_lanes<kWaves>(k);
-  const float group = over_group(m, lanes, larger<float>);
-  const float least = over_group(group, kWaveSize, smaller<float>);
-  m = wave_max(group);
-  if (lane == 0) {
-    s_max[wave] = m;
-    s_bound[wave] = least;
-  }
+  s_max[tid] = m;
   __syncthreads();
-  float bound = s_bound[0];
-  m = s_max[0];
+  float top[kWaves], of_lane[1];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) {
-    m = fmaxf(m, s_max[w]);
-    bound = fminf(bound, s_bound[w]);
+  for (int w = 0; w < kWaves; ++w) top[w] = s_max[w * kWaveSize + lane];
+  of_lane[0] = top[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) of_lane[0] = fmaxf(of_lane[0], top[w]);
+  m = wave_reduce_max(of_lane[0]);
+  // sixteen bits of the order are a bf16 value's, and as near as 2^-7 to others
+  float bound = m;
+  if (k > 1) {
+    u32 order = k <= kWaveSize ? reached_by<16>(of_lane, k)
+                               : reached_by<16>(top, k);
+    if (sizeof(A) == 2 && !(order >> 31)) order |= 0xffffu;
+    bound = value_of(order);
   }
-  if (k == 1) bound = m;
   // -inf is no candidate
   bound = fmaxf(bound, -3.402823466e38f);
   const float from = m == -INFINITY ? 0.f : m;
+  // logits are taken apart again: kept, they would leave a SIMD three waves
+#pragma unroll
+  for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(raw[i]));
 
   double sum = 0.0;
   int held = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     unpack(raw[i], x, row);
-    float e2[L];
+    if (k && __ballot(piece[i] >= bound)) {
+#pragma unroll
+      for (int e = 0; e < L; ++e) {
+        const u64 reach = __ballot(x[e] >= bound);
+        if (reach) {
+          const int at = held + __popcll(reach & below);
+          if (x[e] >= bound && at < kHeld)
+            s_key[wave][at] = key_of(x[e], (first + i * kThreads) * L + e);
+          held += __popcll(reach);
+        }
+      }
+    }
 #pragma unroll
     for (int e = 0; e < L; ++e)
-      e2[e] = __builtin_amdgcn_exp2f((x[e] - from) * kLog2e);
+      x[e] = __builtin_amdgcn_exp2f((x[e] - from) * kLog2e);
 #pragma unroll
     for (int n = L / 2; n; n >>= 1)
 #pragma unroll
-      for (int e = 0; e < n; ++e) e2[e] += e2[e + n];
-    sum += static_cast<double>(e2[0]);
-    if (k == 0) continue;
-#pragma unroll
-    for (int e = 0; e < L; ++e) {
-      const u64 reach = __ballot(x[e] >= bound);
-      if (reach) {
-        const int at = held + __popcll(reach & ((1ull << lane) - 1));
-        if (x[e] >= bound && at < kHeld)
-          s_key[wave][at] =
-              key_of(x[e], (first + i * kThreads) * L + e);
-        held += __popcll(reach);
-      }
-    }
+      for (int e = 0; e < n; ++e) x[e] += x[e + n];
+    sum += static_cast<double>(x[0]);
   }
-  sum = over_group(sum, kWaveSize, [](double a, double b) { return a + b; });
+  sum = wave_sum(sum);
   if (lane == 0) {
     s_sum[wave] = sum;
     s_count[wave] = held;
@@ -265,52 +273,93 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
   }
   if (k == 0) return;
 
-  u64* out = keys + static_cast<int64_t>(blockIdx.x) * k;
-  int all = 0, most = 0;
+  int most = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    all += s_count[w];
-    most = max(most, s_count[w]);
-  }
-  if (most <= kHeld && k <= kThreads) {
-    for (int i = tid; i < all; i += kThreads) {
-      int w = 0, at = i;
-      while (at >= s_count[w]) at -= s_count[w++];
-      const u64 mine = s_key[w][at];
-      int rank = 0;
-      for (int v = 0; v < kWaves; ++v) {
-        const int n = s_count[v];
-        for (int j = 0; j < n; ++j) rank += s_key[v][j] > mine;
+  for (int w = 0; w < kWaves; ++w) most = max(most, s_count[w]);
+  if (most > kHeld) {
+    // Many equal logits, or large ones in few of the groups. The bound becomes
+    // the k-th largest logit, and those that equal it are taken by index, in
+    // each wave up to the k-th.
+    const auto above = [&](float v) {
+      int count = 0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        unpack(raw[i], x, row);
+#pragma unroll
+        for (int e = 0; e < L; ++e) count += __popcll(__ballot(x[e] > v));
       }
-      if (rank < k) out[rank] = mine;
+      __syncthreads();
+      if (lane == 0) s_count[wave] = count;
+      __syncthreads();
+      count = 0;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) count += s_count[w];
+      return count;
+    };
+    if (sizeof(A) == 4 && k > 1)
+      bound = fmaxf(bound, value_of(k <= kWaveSize ? reached_by<0>(of_lane, k)
+                                                   : reached_by<0>(top, k)));
+    if (above(bound) >= k) {
+      u32 lo = order_of(bound), hi = order_of(m);
+      while (hi - lo > 1) {
+        const u32 mid = lo + (hi - lo) / 2;
+        if (above(value_of(mid)) >= k)
+          lo = mid;
+        else
+          hi = mid;
+      }
+      bound = value_of(hi);
     }
-    for (int i = all + tid; i < k; i += kThreads) out[i] = 0;
-    return;
-  }
-  u64 last = ~0ull;
-  for (int n = 0; n < k; ++n) {
-    u64 best = 0;
+    int equal = 0;
+    held = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       unpack(raw[i], x, row);
+      u64 same[L];
+      int rank = equal;
 #pragma unroll
       for (int e = 0; e < L; ++e) {
-        const u64 key = key_of(x[e], (first + i * kThreads) * L + e);
-        if (x[e] > -INFINITY && key < last && key > best) best = key;
+        same[e] = __ballot(x[e] == bound);
+        equal += __popcll(same[e]);
+        rank += __popcll(same[e] & below);
+      }
+#pragma unroll
+      for (int e = 0; e < L; ++e) {
+        const bool take = x[e] > bound || (x[e] == bound && rank < k);
+        rank += x[e] == bound;
+        const u64 taken = __ballot(take);
+        if (take)
+          s_key[wave][held + __popcll(taken & below)] =
+              key_of(x[e], (first + i * kThreads) * L + e);
+        held += __popcll(taken);
       }
     }
-    best = wave_max(best);
     __syncthreads();
-    if (lane == 0) s_key[wave][0] = best;
+    if (lane == 0) s_count[wave] = held;
     __syncthreads();
-    for (int w = 0; w < kWaves; ++w) best = larger(best, s_key[w][0]);
-    if (tid == 0) out[n] = best;
-    last = best;
-    if (!best) {
-      for (int i = n + 1 + tid; i < k; i += kThreads) out[i] = 0;
-      return;
-    }
   }
+
+  // [search, place, beam, chunk]
+  const int64_t g = r / B;
+  const int lists = B * chunks;
+  u64* out = keys + g * k * lists + (blockIdx.x - g * lists);
+  int all = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) all += s_count[w];
+  for (int i = tid; i < all; i += kThreads) {
+    int w = 0, at = i;
+    while (at >= s_count[w]) at -= s_count[w++];
+    const u64 mine = s_key[w][at];
+    int rank = 0;
+    for (int v = 0; v < kWaves; ++v) {
+      const int n = s_count[v];
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) rank += s_key[v][j] > mine;
+    }
+    if (rank < k) out[static_cast<int64_t>(rank) * lists] = mine;
+  }
+  for (int i = all + tid; i < k; i += kThreads)
+    out[static_cast<int64_t>(i) * lists] = 0;
 }
 
 // A candidate: its score's order, its beam, its key; none has score 0.
@@ -351,88 +400,124 @@ struct RowSum {
 FI_DEV RowSum join_sums(const ChunkSum* sums, int chunks, int lane) {
   float m = -INFINITY;
   for (int c = lane; c < chunks; c += kWaveSize) m = fmaxf(m, sums[c].m);
-  m = wave_max(m);
+  m = wave_reduce_max(m);
   const double from = m == -INFINITY ? 0.0 : m;
   double s = 0.0;
   for (int c = lane; c < chunks; c += kWaveSize)
     s += sums[c].s * exp(sums[c].m - from);
-  s = over_group(s, kWaveSize, [](double a, double b) { return a + b; });
-  return {log(s), m};
+  return {log(wave_sum(s)), m};
 }
 
-constexpr int kJoined = 192;  // of a wave, in LDS
-
-// The first k of N choices, `at(i)` the i-th one, to put(place, choice); places
-// that no choice fills get one of score 0.
-template <int WAVES, class At, class Put>
-FI_DEV void first_choices(const int N, const int k, At at, Put put) {
-  __shared__ u64 s_bound[WAVES];
-  __shared__ int s_count[WAVES];
-  __shared__ Choice s_choice[WAVES][kJoined];
+// The first k of the choices that `lists` lists hold, `each` of them in order:
+// key(i) is that of place i / lists of list i % lists, 0 beyond a list's end,
+// and choice(i, key) the choice. To put(place, choice); places that no choice
+// fills get one of score 0.
+//
+// A thread reads its first kAhead keys at once, before sums() joins the rows'
+// sums: a join is one workgroup's chain of waits. The bound is found from the
+// threads' best ones, beginning with the lists' first. Further places are read
+// in turn until one of all lists holds nothing that reaches it.
+constexpr int kAhead = 8;
+template <int WAVES, class Key, class Sums, class Of, class Put>
+FI_DEV void first_choices(const int lists, const int each, const int k,
+                          Key key, Sums sums, Of choice, Put put) {
   constexpr int T = WAVES * kWaveSize;
+  __shared__ __attribute__((aligned(16))) u64 s_top[T];
+  __shared__ u64 s_bound;
+  __shared__ int s_count, s_reached[2];
+  __shared__ Choice s_choice[2 * T];
   const int tid = threadIdx.x, lane = tid % kWaveSize;
-  const int wave = __builtin_amdgcn_readfirstlane(tid / kWaveSize);
-  int all = 0, most = kJoined + 1;
-  if (k <= T) {
-    u64 top = 0;
-    for (int i = tid; i < N; i += T) top = larger(top, at(i).score);
-    const int lanes = group_lanes<WAVES>(k);
-    top = over_group(top, lanes, larger<u64>);
-    top = over_group(top, kWaveSize, smaller<u64>);
-    if (lane == 0) s_bound[wave] = top;
-    __syncthreads();
-    u64 bound = s_bound[0];
-    for (int w = 1; w < WAVES; ++w) bound = smaller(bound, s_bound[w]);
-    bound = larger<u64>(bound, 1);
-    int held = 0;
-    for (int i0 = wave * kWaveSize; i0 < N; i0 += T) {
-      const int i = i0 + lane;
-      Choice c{0, 0, 0};
-      if (i < N) c = at(i);
-      const u64 reach = __ballot(c.score >= bound);
-      const int to = held + __popcll(reach & ((1ull << lane) - 1));
-      if (c.score >= bound && to < kJoined) s_choice[wave][to] = c;
-      held += __popcll(reach);
+  const int N = lists * each;
+  u64 ahead_keys[kAhead];
+#pragma unroll
+  for (int n = 0; n < kAhead; ++n)
+    ahead_keys[n] = tid + n * T < N ? key(tid + n * T) : 0;
+  if (tid < 2) s_reached[tid] = 0;
+  if (tid == 0) s_count = 0;
+  sums();
+  Choice first[kAhead];
+  u64 top = 0;
+#pragma unroll
+  for (int n = 0; n < kAhead; ++n) {
+    first[n] = {0, 0, 0};
+    if (n * T < N) first[n] = choice(tid + n * T, ahead_keys[n]);
+    top = larger(top, first[n].score);
+  }
+  s_top[tid] = top;
+  __syncthreads();
+  int rank = 0;
+#pragma unroll 8
+  for (int j = 0; j < T; ++j) {
+    const u64 other = s_top[j];
+    rank += other > top || (other == top && j < tid);
+  }
+  if (rank == k - 1) s_bound = larger<u64>(top, 1);
+  __syncthreads();
+  const u64 bound = s_bound;
+  const auto take = [&](const Choice& c, int step) {
+    const u64 reach = __ballot(c.score >= bound);
+    if (!reach) return;
+    int at = 0;
+    if (lane == 0) {
+      at = atomicAdd(&s_count, __popcll(reach));
+      s_reached[step % 2] = step + 1;
     }
-    if (lane == 0) s_count[wave] = held;
-    __syncthreads();
-    most = 0;
-    for (int w = 0; w < WAVES; ++w) {
-      all += s_count[w];
-      most = max(most, s_count[w]);
+    at = __builtin_amdgcn_readfirstlane(at) +
+         __popcll(reach & ((1ull << lane) - 1));
+    if (c.score >= bound && at < 2 * T) s_choice[at] = c;
+  };
+#pragma unroll
+  for (int n = 0; n < kAhead; ++n) take(first[n], 0);
+  // places of all lists, and several a thread
+  const int step = (max(lists, 4 * T) + T - 1) / T * T;
+  for (int from = kAhead * T, n = 0; from < N; from += step) {
+    if (from >= lists) {
+      __syncthreads();
+      if (s_reached[n % 2] != n + 1) break;
+      ++n;
+    }
+    const int to = min(from + step, N);
+    for (int i0 = from; i0 < to; i0 += T) {
+      const int i = i0 + tid;
+      take(i < to ? choice(i, key(i)) : Choice{0, 0, 0}, n);
     }
   }
-  if (most <= kJoined) {
+  __syncthreads();
+  const int all = s_count;
+  if (all <= 2 * T) {
     for (int i = tid; i < all; i += T) {
-      int w = 0, j = i;
-      while (j >= s_count[w]) j -= s_count[w++];
-      const Choice mine = s_choice[w][j];
-      int rank = 0;
-      for (int v = 0; v < WAVES; ++v) {
-        const int n = s_count[v];
-        for (int q = 0; q < n; ++q) rank += ahead(s_choice[v][q], mine);
+      const Choice mine = s_choice[i];
+      int place = 0;
+#pragma unroll 4
+      for (int j = 0; j < all; ++j) {
+        const u64 other = s_choice[j].score;
+        if (other == mine.score)
+          place += ahead(s_choice[j], mine);
+        else
+          place += other > mine.score;
       }
-      if (rank < k) put(rank, mine);
+      if (place < k) put(place, mine);
     }
     for (int i = all + tid; i < k; i += T) put(i, Choice{0, 0, 0});
     return;
   }
+  // more equal ones than fit: a round of the workgroup each
   Choice last{~0ull, 0, -1};
   for (int n = 0; n < k; ++n) {
     Choice best{0, 0, 0};
     if (last.score)
       for (int i = tid; i < N; i += T) {
-        const Choice c = at(i);
+        const Choice c = choice(i, key(i));
         if (c.score && ahead(last, c) && ahead(c, best)) best = c;
       }
-    best = over_group(best, kWaveSize, [](const Choice& a, const Choice& b) {
+    best = over_wave(best, [](const Choice& a, const Choice& b) {
       return ahead(b, a) ? b : a;
     });
     __syncthreads();
-    if (lane == 0) s_choice[wave][0] = best;
+    if (lane == 0) s_choice[tid / kWaveSize] = best;
     __syncthreads();
     for (int w = 0; w < WAVES; ++w)
-      if (ahead(s_choice[w][0], best)) best = s_choice[w][0];
+      if (ahead(s_choice[w], best)) best = s_choice[w];
     if (tid == 0) put(n, best);
     last = best;
   }
@@ -448,23 +533,24 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(
   __shared__ RowSum s_row[kMostBeams];
   __shared__ float s_score[kMostBeams];
   const int64_t g = blockIdx.x;
-  const int lane = threadIdx.x % kWaveSize;
-  for (int b = threadIdx.x / kWaveSize; b < B; b += kWaves) {
-    const RowSum z = join_sums(sums + (g * B + b) * chunks, chunks, lane);
-    if (lane == 0) {
-      s_row[b] = z;
-      const float c = scores[g * group_stride + b * beam_stride];
-      s_score[b] = z.alive() ? c : NAN;
-    }
-  }
-  __syncthreads();
-  const int of_beam = chunks * each;
-  keys += g * B * of_beam;
+  const int lists = B * chunks;
+  keys += g * lists * each;
   first_choices<kWaves>(
-      B * of_beam, k,
-      [&](int i) -> Choice {
-        const u64 key = keys[i];
-        const int b = i / of_beam;
+      lists, each, k, [&](int i) { return keys[i]; },
+      [&] {
+        const int lane = threadIdx.x % kWaveSize;
+        for (int b = threadIdx.x / kWaveSize; b < B; b += kWaves) {
+          const RowSum z = join_sums(sums + (g * B + b) * chunks, chunks, lane);
+          if (lane == 0) {
+            s_row[b] = z;
+            const float c = scores[g * group_stride + b * beam_stride];
+            s_score[b] = z.alive() ? c : NAN;
+          }
+        }
+        __syncthreads();
+      },
+      [&](int i, u64 key) -> Choice {
+        const int b = i % lists / chunks;
         const double c = s_score[b];
         if (!key || !finite(c)) return {0, 0, 0};
         return {score_order(c + s_row[b].of(value_of(key >> 32))), key, b};
@@ -491,41 +577,43 @@ __global__ __launch_bounds__(WAVES * kWaveSize) void top_join_kernel(
   const int64_t r = blockIdx.x;
   const int tid = threadIdx.x, lane = tid % kWaveSize;
   const A* row = logits + r * stride;
-  const RowSum z = join_sums(sums + r * chunks, chunks, lane);
-  const bool some = z.alive();
-  if (out_given && tid == 0) {
+  float of = -INFINITY;
+  bool inside = false;
+  if (out_given) {
     const int64_t t = given[r];
-    float v = -INFINITY;
-    if (t >= 0 && t < V) v = z.of(logit_of(row + t));
-    out_given[r] = some ? v : NAN;
+    inside = t >= 0 && t < V;
+    if (inside) of = logit_of(row + t);
   }
-  if (k == 0) return;
-  out_lp += r * k;
-  out_ids += r * k;
-  if (!some) {
-    for (int i = tid; i < k; i += WAVES * kWaveSize) {
-      out_lp[i] = NAN;
-      out_ids[i] = i;
-    }
+  RowSum z;
+  const auto join = [&] {
+    z = join_sums(sums + r * chunks, chunks, lane);
+    if (out_given && tid == 0)
+      out_given[r] = !z.alive() ? NAN : inside ? z.of(of) : -INFINITY;
+  };
+  if (k == 0) {
+    join();
     return;
   }
+  out_lp += r * k;
+  out_ids += r * k;
   keys += r * chunks * k;
   __shared__ int s_found;
   if (tid == 0) s_found = k;
-  __syncthreads();
   // by the keys alone: two log-probabilities may round to one
   first_choices<WAVES>(
-      chunks * k, k,
-      [&](int i) -> Choice {
-        const u64 key = keys[i];
-        return {key, key, 0};
+      chunks, k, k, [&](int i) { return keys[i]; }, join,
+      [&](int, u64 key) -> Choice {
+        return {z.alive() ? key : 0, key, 0};
       },
       [&](int i, const Choice& c) {
         if (c.score) {
           out_lp[i] = z.of(value_of(c.key >> 32));
           out_ids[i] = token_of(c.key);
-        } else {
+        } else if (z.alive()) {
           atomicMin(&s_found, i);
+        } else {
+          out_lp[i] = NAN;
+          out_ids[i] = i;
         }
       });
   __syncthreads();
@@ -572,7 +660,7 @@ int64_t logit_workspace(int64_t R, int V, int k, int size) {
 
 template <typename A>
 static Cut launch_logit_chunks(const A* logits, int64_t stride, int64_t R,
-                               int V, int k, void* workspace,
+                               int V, int B, int k, void* workspace,
                                hipStream_t stream) {
   const Cut cut = cut_of(R, V, sizeof(A));
   ChunkSum* sums = static_cast<ChunkSum*>(workspace);
@@ -580,8 +668,8 @@ static Cut launch_logit_chunks(const A* logits, int64_t stride, int64_t R,
   const dim3 grid(R * cut.chunks);
 #define FI_CHUNKS(NV)                                                      \
   hipLaunchKernelGGL((logit_chunks_kernel<A, NV>), grid, dim3(kThreads), 0, \
-                     stream, logits, stride, V, cut.chunks, cut.vc, k, sums, \
-                     keys)
+                     stream, logits, stride, V, cut.chunks, cut.vc, B, k,    \
+                     sums, keys)
   if (cut.nv == 8)
     FI_CHUNKS(8);
   else if (cut.nv == 4)
@@ -602,7 +690,7 @@ void launch_beam_select(const A* logits, int64_t stride, int V,
                         int* out_tokens, hipStream_t stream) {
   const int each = std::min(k, V);
   const Cut cut =
-      launch_logit_chunks(logits, stride, G * B, V, each, workspace, stream);
+      launch_logit_chunks(logits, stride, G * B, V, B, each, workspace, stream);
   const ChunkSum* sums = static_cast<const ChunkSum*>(workspace);
   hipLaunchKernelGGL(
       beam_join_kernel, dim3(G), dim3(kThreads), 0, stream, sums,
@@ -617,8 +705,8 @@ static void launch_top_join(const A* logits, int64_t stride, int64_t R, int V,
                             const ChunkSum* sums, float* out_lp, int* out_ids,
                             float* out_given, hipStream_t stream) {
   const u64* keys = reinterpret_cast<const u64*>(sums + R * cut.chunks);
-  // a wave finds up to 64 in one go
-  if (k <= kWaveSize && cut.chunks * k <= 512)
+  // a wave's threads hold up to 512 of them at once
+  if (k <= kWaveSize && cut.chunks * k <= kAhead * kWaveSize)
     hipLaunchKernelGGL((top_join_kernel<A, I, 1>), dim3(R), dim3(kWaveSize), 0,
                        stream, logits, stride, V, sums, keys, cut.chunks, k,
                        given, out_lp, out_ids, out_given);
@@ -634,7 +722,7 @@ void launch_top_logprobs(const A* logits, int64_t stride, int64_t R, int V,
                          float* out_lp, int* out_ids, float* out_given,
                          hipStream_t stream) {
   const Cut cut =
-      launch_logit_chunks(logits, stride, R, V, k, workspace, stream);
+      launch_logit_chunks(logits, stride, R, V, 1, k, workspace, stream);
   const ChunkSum* sums = static_cast<const ChunkSum*>(workspace);
   if (wide)
     launch_top_join(logits, stride, R, V, cut, k,

@@ -29,34 +29,39 @@ void check_launch() {
   TORCH_CHECK(e == hipSuccess, "launch failed: ", hipGetErrorString(e));
 }
 
-void check_logits(const at::Tensor& t) {
-  TORCH_CHECK(t.is_cuda() && t.dim() == 2 &&
-                  (t.scalar_type() == at::kFloat ||
-                   t.scalar_type() == at::kBFloat16),
-              "logits must be float32 or bfloat16 rows on the GPU");
-  // a grid holds 2^32 threads, some dozen workgroups a row
-  TORCH_CHECK(t.size(1) >= 1 && t.size(1) < (1ll << 30) &&
-                  t.size(0) * t.size(1) / 2048 + t.size(0) < (1ll << 23),
-              "too many logits in one call");
-  TORCH_CHECK(t.stride(1) == 1 || t.size(1) == 1,
-              "the tokens of a row of logits must follow one another");
+// Checks raise ValueError, as those of CPU operands do.
+#define CHECK_THAT(ok, ...) TORCH_CHECK_VALUE(ok, __VA_ARGS__)
+
+// rows with their tokens one after another
+at::Tensor rows_of(const at::Tensor& t) {
+  CHECK_THAT(t.is_cuda() && t.dim() == 2 && t.size(1) >= 1,
+             "logits are rows of at least one token");
+  CHECK_THAT(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16,
+             "logits are float32 or bfloat16");
+  // a grid holds 2^32 threads, at most one workgroup for 1024 logits or row
+  CHECK_THAT(t.size(1) < (1ll << 30) &&
+                 t.size(0) * (t.size(1) / 1024 + 1) < (1ll << 24),
+             "too many logits in one call");
+  if (t.stride(1) == 1 || t.size(1) == 1) return t;
+  return t.contiguous();
 }
 
 // scores [G, k], parents [G, k], tokens [G, k]
 std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_select(
-    const at::Tensor& logits, const at::Tensor& scores, int64_t k) {
-  check_logits(logits);
-  TORCH_CHECK(k >= 1 && k <= fi::kMostChoices, "k out of range");
-  TORCH_CHECK(scores.dim() == 2 && scores.scalar_type() == at::kFloat &&
-                  scores.device() == logits.device(),
-              "scores must be float32 [searches, beams] beside the logits");
+    const at::Tensor& of, const at::Tensor& scores, int64_t k) {
+  const at::Tensor logits = rows_of(of);
+  CHECK_THAT(k >= 1 && k <= fi::kMostChoices, "k is ", k, ", not from 1 to ",
+             fi::kMostChoices);
+  CHECK_THAT(scores.dim() == 2 && scores.scalar_type() == at::kFloat &&
+                 scores.device() == logits.device(),
+             "scores are float32 [searches, beams] on the device of the "
+             "logits");
   const int64_t G = scores.size(0), B = scores.size(1);
-  TORCH_CHECK(G * B == logits.size(0) && (B >= 1 || G == 0) &&
-                  B <= fi::kMostBeams,
-              "one row of logits per beam");
-  // choices of a search are counted in 32 bits
-  TORCH_CHECK((logits.size(1) / 1024 + 2) * B * k < (1ll << 31),
-              "too many logits and choices in one search");
+  CHECK_THAT(G * B == logits.size(0) && B >= 1 && B <= fi::kMostBeams,
+             logits.size(0), " rows of logits for [", G, ", ", B, "] beams");
+  // the choices of a search are counted in 32 bits
+  CHECK_THAT((logits.size(1) / 1024 + 1) * B * k < (1ll << 31),
+             "too many logits and choices in one search");
   const Guard guard(logits.device());
   const auto f32 = logits.options().dtype(at::kFloat);
   const auto i32 = logits.options().dtype(at::kInt);
@@ -84,18 +89,22 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_select(
 
 // log-probabilities [R, k], tokens [R, k], of the given tokens [R]
 std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>> top_logprobs(
-    const at::Tensor& logits, int64_t k,
-    const c10::optional<at::Tensor>& given) {
-  check_logits(logits);
+    const at::Tensor& from, int64_t k,
+    const c10::optional<at::Tensor>& token_ids) {
+  const at::Tensor logits = rows_of(from);
   const int64_t R = logits.size(0);
-  TORCH_CHECK(k >= 0 && k <= fi::kMostChoices && k <= logits.size(1),
-              "k out of range");
-  if (given)
-    TORCH_CHECK(given->device() == logits.device() && given->dim() == 1 &&
-                    given->size(0) == R && given->is_contiguous() &&
-                    (given->scalar_type() == at::kInt ||
-                     given->scalar_type() == at::kLong),
-                "token_ids must be int32 or int64 [rows] beside the logits");
+  const int64_t most = std::min<int64_t>(fi::kMostChoices, logits.size(1));
+  CHECK_THAT(k >= 0 && k <= most, "k is ", k, ", not from 0 to ", most);
+  c10::optional<at::Tensor> given;
+  if (token_ids) {
+    CHECK_THAT(token_ids->device() == logits.device() &&
+                   token_ids->dim() == 1 && token_ids->size(0) == R &&
+                   (token_ids->scalar_type() == at::kInt ||
+                    token_ids->scalar_type() == at::kLong),
+               "token_ids are int32 or int64, one for each row, on its "
+               "device");
+    given = token_ids->contiguous();
+  }
   const Guard guard(logits.device());
   const auto f32 = logits.options().dtype(at::kFloat);
   at::Tensor lp = at::empty({R, k}, f32);
@@ -123,32 +132,34 @@ std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>> top_logprobs(
   return {lp, ids, of};
 }
 
-void copy_blocks(const std::vector<at::Tensor>& tensors, const at::Tensor& src,
-                 const at::Tensor& dst,
-                 const c10::optional<at::Tensor>& tokens) {
-  TORCH_CHECK(src.is_cuda() && src.scalar_type() == at::kInt &&
-                  src.dim() == 1 && src.is_contiguous(),
-              "src must be int32 ids on the GPU");
-  const int64_t pairs = src.numel();
-  const auto ids = [&](const at::Tensor& t, const char* what) {
-    TORCH_CHECK(t.device() == src.device() && t.scalar_type() == at::kInt &&
-                    t.dim() == 1 && t.is_contiguous() && t.numel() == pairs,
-                what, " must be int32, one for each of src, beside it");
+void copy_blocks(const std::vector<at::Tensor>& tensors,
+                 const at::Tensor& src_ids, const at::Tensor& dst_ids,
+                 const c10::optional<at::Tensor>& token_counts) {
+  const int64_t pairs = src_ids.numel();
+  const auto ids = [&](const at::Tensor& t) {
+    CHECK_THAT(t.scalar_type() == at::kInt,
+               "src, dst and tokens are int32");
+    CHECK_THAT(t.dim() == 1 && t.numel() == pairs,
+               "src, dst and tokens hold one value for each pair");
+    CHECK_THAT(t.is_cuda() && t.device() == src_ids.device(),
+               "tensors and ids are on one device");
+    return t.contiguous();
   };
-  ids(dst, "dst");
-  if (tokens) ids(*tokens, "tokens");
-  TORCH_CHECK(pairs < (1ll << 31), "too many pairs");
+  const at::Tensor src = ids(src_ids), dst = ids(dst_ids);
+  c10::optional<at::Tensor> tokens;
+  if (token_counts) tokens = ids(*token_counts);
+  CHECK_THAT(pairs < (1ll << 31), "too many pairs");
   int block_size = -1;
   for (const auto& t : tensors) {
-    TORCH_CHECK(t.device() == src.device() && t.dim() >= 1 &&
-                    t.is_contiguous(),
-                "tensors of blocks must be contiguous and beside src");
+    CHECK_THAT(t.dim() >= 1 && t.is_contiguous(),
+               "tensors of blocks are contiguous");
+    CHECK_THAT(t.device() == src.device(),
+               "tensors and ids are on one device");
     if (!tokens) continue;
-    TORCH_CHECK(t.dim() == 4,
-                "tokens go with paged tensors [blocks, heads, tokens, width]");
-    TORCH_CHECK(block_size < 0 || t.size(2) == block_size,
-                "paged tensors of one call have blocks of one size");
-    TORCH_CHECK(t.size(2) < (1ll << 31), "too many tokens in a block");
+    CHECK_THAT(t.dim() == 4 && t.size(2) < (1ll << 31) &&
+                   (block_size < 0 || t.size(2) == block_size),
+               "tokens go with paged tensors [blocks, heads, block_size, "
+               "width] of one block_size");
     block_size = static_cast<int>(t.size(2));
   }
   if (pairs == 0) return;
@@ -169,7 +180,7 @@ void copy_blocks(const std::vector<at::Tensor>& tensors, const at::Tensor& src,
     const int64_t block = t.numel() / t.size(0) * t.element_size();
     const int64_t heads = tokens ? t.size(1) : 1;
     const int64_t token = tokens ? t.size(3) * t.element_size() : block;
-    TORCH_CHECK(block < (1ll << 31) && t.size(0) < (1ll << 31),
+    CHECK_THAT(block < (1ll << 31) && t.size(0) < (1ll << 31),
                 "a block must be smaller than 2 GiB");
     const auto bits =
         reinterpret_cast<uintptr_t>(t.data_ptr()) | block | token;
