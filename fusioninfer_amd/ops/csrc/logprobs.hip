@@ -126,13 +126,11 @@ struct alignas(16) ChunkSum {
 
 constexpr int kHeld = 320;  // of a wave, in LDS
 
-// The order of the k-th largest of the wave's N * 64 values, from its upper
-// bits down to bit LAST; the others are 0.
+// The k-th largest of the wave's N * 64 orders, from its upper bits down to bit
+// LAST; the others are 0.
 template <int LAST, int N>
-FI_DEV u32 reached_by(const float (&v)[N], int k) {
-  u32 order[N], bound = 0;
-#pragma unroll
-  for (int i = 0; i < N; ++i) order[i] = order_of(v[i]);
+FI_DEV u32 reached_by(const u32 (&order)[N], int k) {
+  u32 bound = 0;
 #pragma unroll
   for (int bit = 31; bit >= LAST; --bit) {
     const u32 next = bound | 1u << bit;
@@ -211,18 +209,22 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
   }
   s_max[tid] = m;
   __syncthreads();
-  float top[kWaves], of_lane[1];
+  // Groups of four threads for small k, a sixteenth more values than k for 16 of
+  // 64 groups, two fifths for 32; then each thread is one.
+  u32 top[kWaves], of_lane[1] = {0};
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) top[w] = s_max[w * kWaveSize + lane];
-  of_lane[0] = top[0];
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) of_lane[0] = fmaxf(of_lane[0], top[w]);
-  m = wave_reduce_max(of_lane[0]);
+  for (int w = 0; w < kWaves; ++w) {
+    const float v = s_max[w * kWaveSize + lane];
+    m = fmaxf(m, v);
+    top[w] = order_of(v);
+    of_lane[0] = larger(of_lane[0], top[w]);
+  }
+  m = wave_reduce_max(m);
+  const bool few = k <= 32;
   // sixteen bits of the order are a bf16 value's, and as near as 2^-7 to others
   float bound = m;
   if (k > 1) {
-    u32 order = k <= kWaveSize ? reached_by<16>(of_lane, k)
-                               : reached_by<16>(top, k);
+    u32 order = few ? reached_by<16>(of_lane, k) : reached_by<16>(top, k);
     if (sizeof(A) == 2 && !(order >> 31)) order |= 0xffffu;
     bound = value_of(order);
   }
@@ -297,8 +299,8 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
       return count;
     };
     if (sizeof(A) == 4 && k > 1)
-      bound = fmaxf(bound, value_of(k <= kWaveSize ? reached_by<0>(of_lane, k)
-                                                   : reached_by<0>(top, k)));
+      bound = fmaxf(bound, value_of(few ? reached_by<0>(of_lane, k)
+                                        : reached_by<0>(top, k)));
     if (above(bound) >= k) {
       u32 lo = order_of(bound), hi = order_of(m);
       while (hi - lo > 1) {
@@ -396,16 +398,34 @@ struct RowSum {
   FI_DEV double of(float v) const { return (static_cast<double>(v) - m) - ln; }
 };
 
-// by one wave, in all of its lanes
-FI_DEV RowSum join_sums(const ChunkSum* sums, int chunks, int lane) {
-  float m = -INFINITY;
-  for (int c = lane; c < chunks; c += kWaveSize) m = fmaxf(m, sums[c].m);
-  m = wave_reduce_max(m);
+// Joined by groups of 16, 32 or 64 lanes, whichever hold the chunks of a row
+// (64 go round), in all of the group's lanes. Rows of sums begin at `sums`.
+FI_DEV int lanes_for(int chunks) {
+  return chunks <= 16 ? 16 : chunks <= 32 ? 32 : kWaveSize;
+}
+template <class T, class Op>
+FI_DEV T over_lanes(T v, int lanes, Op op) {
+  if (lanes > 32) v = op(v, partner<32>(v));
+  if (lanes > 16) v = op(v, partner<16>(v));
+  v = op(v, partner<8>(v));
+  v = op(v, partner<4>(v));
+  v = op(v, partner<2>(v));
+  return op(v, partner<1>(v));
+}
+FI_DEV RowSum join_sums(const ChunkSum* sums, int chunks, int lanes) {
+  const int at = threadIdx.x & (lanes - 1);
+  ChunkSum own{0.0, -INFINITY};
+  if (at < chunks) own = sums[at];
+  float m = own.m;
+  for (int c = at + kWaveSize; c < chunks; c += kWaveSize)
+    m = fmaxf(m, sums[c].m);
+  m = over_lanes(m, lanes, larger<float>);
   const double from = m == -INFINITY ? 0.0 : m;
-  double s = 0.0;
-  for (int c = lane; c < chunks; c += kWaveSize)
+  double s = own.s * exp(own.m - from);
+  for (int c = at + kWaveSize; c < chunks; c += kWaveSize)
     s += sums[c].s * exp(sums[c].m - from);
-  return {log(wave_sum(s)), m};
+  s = over_lanes(s, lanes, [](double a, double b) { return a + b; });
+  return {log(s), m};
 }
 
 // The first k of the choices that `lists` lists hold, `each` of them in order:
@@ -422,8 +442,7 @@ template <int WAVES, class Key, class Sums, class Of, class Put>
 FI_DEV void first_choices(const int lists, const int each, const int k,
                           Key key, Sums sums, Of choice, Put put) {
   constexpr int T = WAVES * kWaveSize;
-  __shared__ __attribute__((aligned(16))) u64 s_top[T];
-  __shared__ u64 s_bound;
+  __shared__ u32 s_top[T];
   __shared__ int s_count, s_reached[2];
   __shared__ Choice s_choice[2 * T];
   const int tid = threadIdx.x, lane = tid % kWaveSize;
@@ -443,17 +462,14 @@ FI_DEV void first_choices(const int lists, const int each, const int k,
     if (n * T < N) first[n] = choice(tid + n * T, ahead_keys[n]);
     top = larger(top, first[n].score);
   }
-  s_top[tid] = top;
+  s_top[tid] = static_cast<u32>(top >> 32);
   __syncthreads();
-  int rank = 0;
-#pragma unroll 8
-  for (int j = 0; j < T; ++j) {
-    const u64 other = s_top[j];
-    rank += other > top || (other == top && j < tid);
-  }
-  if (rank == k - 1) s_bound = larger<u64>(top, 1);
-  __syncthreads();
-  const u64 bound = s_bound;
+  u32 tops[WAVES];
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) tops[w] = s_top[w * kWaveSize + lane];
+  // upper halves of the scores' orders: twenty bits of mantissa
+  const u64 bound =
+      larger<u64>(static_cast<u64>(reached_by<0>(tops, k)) << 32, 1);
   const auto take = [&](const Choice& c, int step) {
     const u64 reach = __ballot(c.score >= bound);
     if (!reach) return;
@@ -538,12 +554,15 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(
   first_choices<kWaves>(
       lists, each, k, [&](int i) { return keys[i]; },
       [&] {
-        const int lane = threadIdx.x % kWaveSize;
-        for (int b = threadIdx.x / kWaveSize; b < B; b += kWaves) {
-          const RowSum z = join_sums(sums + (g * B + b) * chunks, chunks, lane);
-          if (lane == 0) {
+        const int lanes = lanes_for(chunks);
+        for (int b0 = 0; b0 < B; b0 += kThreads / lanes) {
+          const int b = b0 + threadIdx.x / lanes;
+          const int in = min(b, B - 1);  // all lanes take part
+          const float c = scores[g * group_stride + in * beam_stride];
+          const RowSum z =
+              join_sums(sums + (g * B + in) * chunks, chunks, lanes);
+          if (b < B && threadIdx.x % lanes == 0) {
             s_row[b] = z;
-            const float c = scores[g * group_stride + b * beam_stride];
             s_score[b] = z.alive() ? c : NAN;
           }
         }
@@ -586,7 +605,7 @@ __global__ __launch_bounds__(WAVES * kWaveSize) void top_join_kernel(
   }
   RowSum z;
   const auto join = [&] {
-    z = join_sums(sums + r * chunks, chunks, lane);
+    z = join_sums(sums + r * chunks, chunks, kWaveSize);
     if (out_given && tid == 0)
       out_given[r] = !z.alive() ? NAN : inside ? z.of(of) : -INFINITY;
   };
