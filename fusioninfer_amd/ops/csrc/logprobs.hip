@@ -48,6 +48,26 @@ FI_DEV void unpack(const u32x4 raw, float (&x)[8], const u16*) {
   }
 }
 
+// Maximum of them and v. The upper logit of a pair is compared as it lies: the
+// lower one's bits follow its own and decide among equal ones alone, or make a
+// NaN of an infinity, which no maximum takes; highest() cuts them off.
+FI_DEV float max_with(const u32x4 raw, float v, const float*) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v = fmaxf(v, __uint_as_float(raw[e]));
+  return v;
+}
+FI_DEV float max_with(const u32x4 raw, float v, const u16*) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    v = fmaxf(v, fmaxf(__uint_as_float(raw[e]),
+                       __uint_as_float(raw[e] << 16)));
+  return v;
+}
+FI_DEV float highest(float v, const float*) { return v; }
+FI_DEV float highest(float v, const u16*) {
+  return __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+}
+
 // order of a finite value; -0 counts as +0
 FI_DEV u32 order_of(float v) {
   const u32 u = __float_as_uint(v + 0.f);
@@ -124,6 +144,17 @@ struct alignas(16) ChunkSum {
   float m;
 };
 
+// exp2(v): as exact as the instruction is on half a power of two
+FI_DEV double power_of_2(double v) {
+  const double whole = rint(v);
+  const float part = __builtin_amdgcn_exp2f(static_cast<float>(v - whole));
+  return whole < -1000.0
+             ? 0.0
+             : ldexp(static_cast<double>(part), static_cast<int>(whole));
+}
+// exp(v), v <= 0
+FI_DEV double power(double v) { return power_of_2(v * 1.4426950408889634); }
+
 constexpr int kHeld = 320;  // of a wave, in LDS
 
 // The k-th largest of the wave's N * 64 orders, from its upper bits down to bit
@@ -171,40 +202,43 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
   const int first = c * VC + tid;
 
   u32x4 raw[NV];
+  // a chunk's first logit, for pieces at 32-bit distances from it
+  const A* from_first = row + static_cast<int64_t>(c) * VC * L;
+  if ((c * VC + NV * kThreads) * L <= V && VC == NV * kThreads) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int j = first + i * kThreads;
-    const u32 none = sizeof(A) == 4 ? 0xff800000u : 0xff80ff80u;
-    raw[i] = u32x4{none, none, none, none};
-    if (j < end && (j + 1) * L <= V)
-      __builtin_memcpy(&raw[i], row + static_cast<int64_t>(j) * L, 16);
-  }
-  if (V % L && (c + 1) * VC >= V / L) {  // the last logits
+    for (int i = 0; i < NV; ++i)
+      __builtin_memcpy(&raw[i], from_first + i * kThreads * L + tid * L, 16);
+  } else {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int j = first + i * kThreads;
-      if (j >= end || j != V / L) continue;
+      const u32 none = sizeof(A) == 4 ? 0xff800000u : 0xff80ff80u;
+      raw[i] = u32x4{none, none, none, none};
+      if (j < end && (j + 1) * L <= V)
+        __builtin_memcpy(&raw[i], row + static_cast<int64_t>(j) * L, 16);
+    }
+    if (V % L && c == chunks - 1) {  // the last logits
+      u32x4 tail = {0, 0, 0, 0};
 #pragma unroll
       for (int e = 0; e < L; ++e) {
-        if (j * L + e >= V) continue;
-        const u32 bits = __float_as_uint(logit_of(row + j * L + e));
+        const int t = V / L * L + e;
+        const u32 bits =
+            t < V ? __float_as_uint(logit_of(row + t)) : 0xff800000u;
         if (sizeof(A) == 4)
-          raw[i][e % 4] = bits;
-        else if (e % 2)
-          raw[i][e / 2] = (raw[i][e / 2] & 0xffffu) | bits;
+          tail[e % 4] = bits;
         else
-          raw[i][e / 2] = (raw[i][e / 2] & 0xffff0000u) | bits >> 16;
+          tail[e / 2] |= e % 2 ? bits : bits >> 16;
       }
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (first + i * kThreads == V / L) raw[i] = tail;
     }
   }
 
   float x[L], piece[NV], m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    unpack(raw[i], x, row);
-    piece[i] = x[0];
-#pragma unroll
-    for (int e = 1; e < L; ++e) piece[i] = fmaxf(piece[i], x[e]);
+    piece[i] = highest(max_with(raw[i], -INFINITY, row), row);
     m = fmaxf(m, piece[i]);
   }
   s_max[tid] = m;
@@ -231,16 +265,47 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
   // -inf is no candidate
   bound = fmaxf(bound, -3.402823466e38f);
   const float from = m == -INFINITY ? 0.f : m;
-  // logits are taken apart again: kept, they would leave a SIMD three waves
-#pragma unroll
-  for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(raw[i]));
 
+  // exp(l - from) in one multiplication and addition, l log2(e) - c. What c is
+  // rounded by is the same for all, and put right below; where it would not be
+  // small beside one the difference comes first.
+  const float c2 = from * kLog2e;
+  const bool near = fabsf(from) <= 32768.f;
+  // Logits are taken apart in each pass anew and a piece at a time: kept, or all
+  // at once, they would leave a SIMD half as many waves.
+  const auto apart = [&](u32x4& of) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __builtin_amdgcn_sched_barrier(0);
+#endif
+    asm volatile("" : "+v"(of));
+    unpack(of, x, row);
+  };
   double sum = 0.0;
-  int held = 0;
+  const auto add_up = [&](auto exponent) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    unpack(raw[i], x, row);
-    if (k && __ballot(piece[i] >= bound)) {
+    for (int i = 0; i < NV; ++i) {
+      apart(raw[i]);
+#pragma unroll
+      for (int e = 0; e < L; ++e)
+        x[e] = __builtin_amdgcn_exp2f(exponent(x[e]));
+#pragma unroll
+      for (int n = L / 2; n; n >>= 1)
+#pragma unroll
+        for (int e = 0; e < n; ++e) x[e] += x[e + n];
+      sum += static_cast<double>(x[0]);
+    }
+  };
+  if (near)
+    add_up([&](float v) { return fmaf(v, kLog2e, -c2); });
+  else
+    add_up([&](float v) { return (v - from) * kLog2e; });
+  asm volatile("" : "+v"(sum));
+  int held = 0;
+  if (k) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (!__ballot(piece[i] >= bound)) continue;
+      apart(raw[i]);
 #pragma unroll
       for (int e = 0; e < L; ++e) {
         const u64 reach = __ballot(x[e] >= bound);
@@ -252,14 +317,6 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
         }
       }
     }
-#pragma unroll
-    for (int e = 0; e < L; ++e)
-      x[e] = __builtin_amdgcn_exp2f((x[e] - from) * kLog2e);
-#pragma unroll
-    for (int n = L / 2; n; n >>= 1)
-#pragma unroll
-      for (int e = 0; e < n; ++e) x[e] += x[e + n];
-    sum += static_cast<double>(x[0]);
   }
   sum = wave_sum(sum);
   if (lane == 0) {
@@ -270,6 +327,8 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
   if (tid == 0) {
     sum = s_sum[0];
     for (int w = 1; w < kWaves; ++w) sum += s_sum[w];
+    if (near)
+      sum *= power_of_2(c2 - static_cast<double>(from) * kLog2e);
     sums[blockIdx.x].s = sum;
     sums[blockIdx.x].m = m;
   }
@@ -286,7 +345,7 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
       int count = 0;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        unpack(raw[i], x, row);
+        apart(raw[i]);
 #pragma unroll
         for (int e = 0; e < L; ++e) count += __popcll(__ballot(x[e] > v));
       }
@@ -316,7 +375,7 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
     held = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      unpack(raw[i], x, row);
+      apart(raw[i]);
       u64 same[L];
       int rank = equal;
 #pragma unroll
@@ -421,9 +480,9 @@ FI_DEV RowSum join_sums(const ChunkSum* sums, int chunks, int lanes) {
     m = fmaxf(m, sums[c].m);
   m = over_lanes(m, lanes, larger<float>);
   const double from = m == -INFINITY ? 0.0 : m;
-  double s = own.s * exp(own.m - from);
+  double s = own.s * power(own.m - from);
   for (int c = at + kWaveSize; c < chunks; c += kWaveSize)
-    s += sums[c].s * exp(sums[c].m - from);
+    s += sums[c].s * power(sums[c].m - from);
   s = over_lanes(s, lanes, [](double a, double b) { return a + b; });
   return {log(s), m};
 }
@@ -470,7 +529,7 @@ FI_DEV void first_choices(const int lists, const int each, const int k,
     tops[w] = s_top[w * kWaveSize + lane];
     of_lane[0] = larger(of_lane[0], tops[w]);
   }
-  // ten bits of mantissa of a score in 64 bits, twelve of a logit
+  // ten bits of mantissa of a score in 64 bits, thirteen of a logit
   const u64 bound = larger<u64>(
       static_cast<u64>(k <= 32 ? reached_by<10>(of_lane, k)
                                : reached_by<10>(tops, k)) << 32, 1);
@@ -694,7 +753,7 @@ Cut cut_of(int64_t R, int V, int size) {
     cut.chunks = (pieces + cut.nv * kThreads - 1) / (cut.nv * kThreads);
     if (cut.nv == 1 || R * cut.chunks >= 64) break;
   }
-  cut.vc = (pieces + cut.chunks - 1) / cut.chunks;
+  cut.vc = cut.nv * kThreads;
   return cut;
 }
 
