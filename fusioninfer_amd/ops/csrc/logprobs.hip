@@ -48,24 +48,14 @@ FI_DEV void unpack(const u32x4 raw, float (&x)[8], const u16*) {
   }
 }
 
-// Maximum of them and v. The upper logit of a pair is compared as it lies: the
-// lower one's bits follow its own and decide among equal ones alone, or make a
-// NaN of an infinity, which no maximum takes; highest() cuts them off.
-FI_DEV float max_with(const u32x4 raw, float v, const float*) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v = fmaxf(v, __uint_as_float(raw[e]));
+// maximum of three; written out, as the compiler first maxes every operand with
+// itself for the sake of signaling NaNs, which leave no distribution anyway
+FI_DEV float max3(float a, float b, float c) {
+  float v = 0.f;
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(v) : "v"(a), "v"(b), "v"(c));
+#endif
   return v;
-}
-FI_DEV float max_with(const u32x4 raw, float v, const u16*) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    v = fmaxf(v, fmaxf(__uint_as_float(raw[e]),
-                       __uint_as_float(raw[e] << 16)));
-  return v;
-}
-FI_DEV float highest(float v, const float*) { return v; }
-FI_DEV float highest(float v, const u16*) {
-  return __uint_as_float(__float_as_uint(v) & 0xffff0000u);
 }
 
 // order of a finite value; -0 counts as +0
@@ -156,6 +146,17 @@ FI_DEV double power_of_2(double v) {
 FI_DEV double power(double v) { return power_of_2(v * 1.4426950408889634); }
 
 constexpr int kHeld = 320;  // of a wave, in LDS
+constexpr int kAtOnce = 8;   // compared without a question between
+
+// how many of n keys, filled up with 0, are ahead
+FI_DEV int ahead_of(const u64* keys, int n, u64 mine) {
+  int count = 0;
+  for (int j = 0; j < n; j += kAtOnce) {
+#pragma unroll
+    for (int q = 0; q < kAtOnce; ++q) count += keys[j + q] > mine;
+  }
+  return count;
+}
 
 // The k-th largest of the wave's N * 64 orders, from its upper bits down to bit
 // LAST; the others are 0.
@@ -191,7 +192,7 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
   __shared__ float s_max[kThreads];
   __shared__ double s_sum[kWaves];
   __shared__ int s_count[kWaves];
-  __shared__ u64 s_key[kWaves][kHeld];
+  __shared__ __attribute__((aligned(16))) u64 s_key[kWaves][kHeld + kAtOnce];
   const int tid = threadIdx.x, lane = tid % kWaveSize;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWaveSize);
   const u64 below = (1ull << lane) - 1;
@@ -238,7 +239,11 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
   float x[L], piece[NV], m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    piece[i] = highest(max_with(raw[i], -INFINITY, row), row);
+    unpack(raw[i], x, row);
+    piece[i] = max3(x[0], x[1], x[2]);
+#pragma unroll
+    for (int e = 3; e < L; e += 2)
+      piece[i] = max3(piece[i], x[e], x[min(e + 1, L - 1)]);
     m = fmaxf(m, piece[i]);
   }
   s_max[tid] = m;
@@ -319,6 +324,7 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
     }
   }
   sum = wave_sum(sum);
+  if (lane < kAtOnce && held <= kHeld) s_key[wave][held + lane] = 0;
   if (lane == 0) {
     s_sum[wave] = sum;
     s_count[wave] = held;
@@ -395,6 +401,7 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
         held += __popcll(taken);
       }
     }
+    if (lane < kAtOnce) s_key[wave][held + lane] = 0;
     __syncthreads();
     if (lane == 0) s_count[wave] = held;
     __syncthreads();
@@ -412,11 +419,8 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
     while (at >= s_count[w]) at -= s_count[w++];
     const u64 mine = s_key[w][at];
     int rank = 0;
-    for (int v = 0; v < kWaves; ++v) {
-      const int n = s_count[v];
-#pragma unroll 4
-      for (int j = 0; j < n; ++j) rank += s_key[v][j] > mine;
-    }
+    for (int v = 0; v < kWaves; ++v)
+      rank += ahead_of(s_key[v], s_count[v], mine);
     if (rank < k) out[static_cast<int64_t>(rank) * lists] = mine;
   }
   for (int i = all + tid; i < k; i += kThreads)
@@ -500,16 +504,19 @@ constexpr int kAhead = 8;
 template <int WAVES, class Key, class Sums, class Of, class Put>
 FI_DEV void first_choices(const int lists, const int each, const int k,
                           Key key, Sums sums, Of choice, Put put) {
-  constexpr int T = WAVES * kWaveSize;
+  constexpr int T = WAVES * kWaveSize, kTaken = 2 * T;
   __shared__ u32 s_top[T];
   __shared__ int s_count, s_reached[2];
-  __shared__ Choice s_choice[2 * T];
+  __shared__ __attribute__((aligned(16))) u64 s_score[kTaken];
+  __shared__ u64 s_key[kTaken];
+  __shared__ int s_beam[kTaken];
   const int tid = threadIdx.x, lane = tid % kWaveSize;
   const int N = lists * each;
   u64 ahead_keys[kAhead];
 #pragma unroll
   for (int n = 0; n < kAhead; ++n)
     ahead_keys[n] = tid + n * T < N ? key(tid + n * T) : 0;
+  for (int i = tid; i < kTaken; i += T) s_score[i] = 0;
   if (tid < 2) s_reached[tid] = 0;
   if (tid == 0) s_count = 0;
   sums();
@@ -551,7 +558,11 @@ FI_DEV void first_choices(const int lists, const int each, const int k,
 #pragma unroll
     for (int n = 0; n < M; ++n) {
       const int to = at + __popcll(reach[n] & ((1ull << lane) - 1));
-      if (of[n].score >= bound && to < 2 * T) s_choice[to] = of[n];
+      if (of[n].score >= bound && to < kTaken) {
+        s_score[to] = of[n].score;
+        s_key[to] = of[n].key;
+        s_beam[to] = of[n].beam;
+      }
       at += __popcll(reach[n]);
     }
   };
@@ -580,18 +591,15 @@ FI_DEV void first_choices(const int lists, const int each, const int k,
   }
   __syncthreads();
   const int all = s_count;
-  if (all <= 2 * T) {
+  if (all <= kTaken) {
     for (int i = tid; i < all; i += T) {
-      const Choice mine = s_choice[i];
-      int place = 0;
-#pragma unroll 4
-      for (int j = 0; j < all; ++j) {
-        const u64 other = s_choice[j].score;
-        if (other == mine.score)
-          place += ahead(s_choice[j], mine);
-        else
-          place += other > mine.score;
-      }
+      const Choice mine{s_score[i], s_key[i], s_beam[i]};
+      int place = ahead_of(s_score, all, mine.score);
+      // itself, and now and then another with its score
+      if (ahead_of(s_score, all, mine.score - 1) != place + 1)
+        for (int j = 0; j < all; ++j)
+          place += s_score[j] == mine.score &&
+                   ahead({mine.score, s_key[j], s_beam[j]}, mine);
       if (place < k) put(place, mine);
     }
     for (int i = all + tid; i < k; i += T) put(i, Choice{0, 0, 0});
@@ -610,16 +618,24 @@ FI_DEV void first_choices(const int lists, const int each, const int k,
       return ahead(b, a) ? b : a;
     });
     __syncthreads();
-    if (lane == 0) s_choice[tid / kWaveSize] = best;
+    if (lane == 0) {
+      s_score[tid / kWaveSize] = best.score;
+      s_key[tid / kWaveSize] = best.key;
+      s_beam[tid / kWaveSize] = best.beam;
+    }
     __syncthreads();
-    for (int w = 0; w < WAVES; ++w)
-      if (ahead(s_choice[w], best)) best = s_choice[w];
+    for (int w = 0; w < WAVES; ++w) {
+      const Choice of{s_score[w], s_key[w], s_beam[w]};
+      if (ahead(of, best)) best = of;
+    }
     if (tid == 0) put(n, best);
     last = best;
   }
 }
 
-// One workgroup per search: the k best of its beams' first tokens.
+// One workgroup per search: the k best of its beams' first tokens. Sixteen waves
+// are slower than four even where 32 beams hand on 16384 keys (29 and 27 us a
+// call).
 __global__ __launch_bounds__(kThreads) void beam_join_kernel(
     const ChunkSum* __restrict__ sums, const u64* __restrict__ keys,
     const int chunks, const float* __restrict__ scores,
@@ -744,7 +760,8 @@ struct Cut {
 // Chunks as large as registers hold, 8 pieces a thread, leave the least to
 // join; halved until 64 workgroups share the call. One search of 4 beams over
 // 151936 tokens 12.3 us so, 14.1 by 256 to 2048 workgroups, which read faster
-// but have twice as much to join; 64 searches of 8 47 us, 49 with 4 pieces.
+// but have twice as much to join; 64 searches of 8 47 us, 49 with 4 pieces. Sixteen
+// pieces are no faster.
 Cut cut_of(int64_t R, int V, int size) {
   const int lanes = 16 / size;
   const int pieces = (V + lanes - 1) / lanes;
