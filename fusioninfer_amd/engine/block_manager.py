@@ -148,6 +148,23 @@ class BlockManager:
             self.ref_count[blk] = 1
             seq.block_ids.append(blk)
 
+    def fork(self, parent: Sequence, child: Sequence, num_tokens: int):
+        """Give `child` the cache of the first num_tokens of `parent`: full
+        blocks are shared, a partly filled last one gets a block of its own.
+        Returns (parent's block, child's block, tokens in it) for the caller
+        to copy, None where all blocks are full."""
+        assert not child.block_ids
+        full, tail = divmod(num_tokens, self.block_size)
+        for blk in parent.block_ids[:full]:
+            self._take(blk)
+            child.block_ids.append(blk)
+        if not tail:
+            return None
+        blk = self._pop_free_block()
+        self.ref_count[blk] = 1
+        child.block_ids.append(blk)
+        return parent.block_ids[full], blk, tail
+
     def free(self, seq: Sequence) -> None:
         for blk in seq.block_ids:
             self.ref_count[blk] -= 1

@@ -14,6 +14,7 @@ from typing import Dict, List, Optional
 
 import torch
 
+import fusioninfer_amd.ops as ops
 from fusioninfer_amd.config import EngineConfig
 from fusioninfer_amd.engine.block_manager import BlockManager
 from fusioninfer_amd.engine.model_runner import ModelRunner
@@ -850,24 +851,37 @@ class LLMEngine:
             if s.sampling.logprobs is not None
         ]
         if lp_rows:
-            lp = torch.log_softmax(logits_f[lp_rows], dim=-1)
-            for j, i in enumerate(lp_rows):
-                s = sample_seqs[i]
-                k = max(int(s.sampling.logprobs), 0)
-                entry_top = {}
-                if k > 0:
-                    vals, idx = lp[j].topk(k)
-                    entry_top = {
-                        int(t): float(v) for t, v in zip(idx, vals)
-                    }
-                s.logprobs.append(
-                    (float(lp[j, next_tokens[i]]), entry_top)
-                )
+            rows = (logits_f if len(lp_rows) == len(sample_seqs)
+                    else logits_f[lp_rows])
+            ks = [max(int(sample_seqs[i].sampling.logprobs), 0)
+                  for i in lp_rows]
+            entries = self._logprob_entries(
+                rows, ks, [next_tokens[i] for i in lp_rows])
+            for i, entry in zip(lp_rows, entries):
+                sample_seqs[i].logprobs.append(entry)
         outputs.extend(
             self._emit_tokens(seq, [tok])
             for seq, tok in zip(sample_seqs, next_tokens)
         )
         return outputs
+
+    def _logprob_entries(self, logits, ks, token_ids):
+        """(log-probability of the given token, {token: log-probability} of
+        the first ks[i] tokens) of every row of logits."""
+        k = min(max(ks), logits.shape[1])
+        if k <= ops.MOST_CHOICES:
+            given = self.runner._to_device(
+                {"ids": (list(token_ids), torch.long)})["ids"]
+            top = ops.top_logprobs(logits, k, given)
+            vals, idx = top.logprobs.tolist(), top.ids.tolist()
+            of = top.token_logprobs.tolist()
+        else:
+            lp = torch.log_softmax(logits, dim=-1)
+            first = lp.topk(k)
+            vals, idx = first.values.tolist(), first.indices.tolist()
+            of = [float(lp[i, t]) for i, t in enumerate(token_ids)]
+        return [(of[i], dict(zip(idx[i][:n], vals[i][:n])))
+                for i, n in enumerate(ks)]
 
     def _consume_prompt_logprobs(self, batch, payload, logits_f,
                                  chunk_starts):
@@ -875,8 +889,9 @@ class LLMEngine:
         logits_rows covering every prompt position of requesting
         sequences; fill seq.prompt_logprobs (index 0 and prefix-cached
         positions are None) and return the standard sampling-row subset
-        in the engine's expected order. log_softmax runs in row slices
-        so a full 8k-token admission never materializes a [T, V] fp32."""
+        in the engine's expected order. Rows are taken in slices: where a
+        slice's log-softmax has to be formed, it is never that of a full
+        8k-token admission."""
         rows = payload["logits_rows"]
         pos_of = {r: i for i, r in enumerate(rows)}
         cu = payload["cu"]
@@ -893,24 +908,16 @@ class LLMEngine:
                     [None] * min(C + 1, seq.num_prompt_tokens)
                 )
             toks = seq.all_token_ids
-            idx = [pos_of[r] for r in range(cu[j], cu[j + 1])]
+            # a sequence's rows follow one another; the last prompt token has
+            # none after it
+            first = pos_of[cu[j]] if n else 0
+            n = min(n, seq.num_prompt_tokens - C - 1)
             for lo in range(0, n, 256):
                 hi = min(lo + 256, n)
-                sub = torch.log_softmax(logits_f[idx[lo:hi]], dim=-1)
-                for i in range(lo, hi):
-                    pos_next = C + i + 1
-                    if pos_next >= seq.num_prompt_tokens:
-                        break
-                    row = sub[i - lo]
-                    entry_top = {}
-                    if k > 0:
-                        vals, tix = row.topk(k)
-                        entry_top = {
-                            int(t): float(v) for t, v in zip(tix, vals)
-                        }
-                    seq.prompt_logprobs.append(
-                        (float(row[toks[pos_next]]), entry_top)
-                    )
+                seq.prompt_logprobs.extend(self._logprob_entries(
+                    logits_f[first + lo: first + hi],
+                    [max(int(k), 0)] * (hi - lo),
+                    toks[C + lo + 1: C + hi + 1]))
         pf_rows = [
             cu[j + 1] - 1 for j, smp in enumerate(payload["sample"]) if smp
         ]
@@ -999,20 +1006,75 @@ class LLMEngine:
         step is decode), longer portions the chunked-prefill segment, and
         the model runner executes them as one mixed batch. Used for
         scoring and for replaying recorded schedules."""
+        self._ready_to_force()
+        if not entries:
+            self.release_forced(end)
+            return torch.empty((0, self.cfg.model.vocab_size))
+        logits, picked = self._forced_rows(entries)
+        # an index that is a list would be copied to the GPU synchronously,
+        # and the host would stand still until this step is over
+        if picked == list(range(logits.shape[0])):
+            out = logits.to(torch.float32, copy=True)
+        else:
+            out = logits.float()[self.runner._to_device(
+                {"rows": (picked, torch.long)})["rows"]]
+        self.release_forced(end)
+        return out
+
+    def forced_logits(self, entries):
+        """forced_step's logits as the model gives them, in its own type; they
+        may lie in a buffer that the next step writes again."""
+        self._ready_to_force()
+        logits, picked = self._forced_rows(entries)
+        if picked == list(range(logits.shape[0])):
+            return logits
+        return logits[self.runner._to_device(
+            {"rows": (picked, torch.long)})["rows"]]
+
+    def release_forced(self, request_ids) -> None:
+        """Give back what requests of forced steps hold; unknown ids are
+        passed over."""
+        for rid in request_ids:
+            seq = self._forced.pop(rid, None)
+            if seq is None:
+                continue
+            self.block_manager.free(seq)
+            if self.state_manager is not None:
+                self.state_manager.free(seq)
+            seq.status = SeqStatus.FINISHED
+
+    def fork_forced(self, request_id: str, child_id: str):
+        """A further request of forced steps that goes on from where another
+        one is. Returns the copies its cache still needs before the next
+        step: (block, block, tokens) or None, and (state slot, state slot) or
+        None."""
+        seq = self._forced[request_id]
+        if child_id in self._forced:
+            raise ValueError(f"request {child_id!r} exists")
+        if seq.num_computed_tokens % self.cfg.cache.block_size \
+                and not self.block_manager.num_free():
+            raise InsufficientBlocksError("a fork needs a cache block, "
+                                          "0 free")
+        child = Sequence(child_id, seq.prompt_token_ids, SamplingParams())
+        child.num_computed_tokens = seq.num_computed_tokens
+        slot = None
+        if self.state_manager is not None:
+            slot = (seq.state_slot, self.state_manager.allocate(child))
+        page = self.block_manager.fork(seq, child, seq.num_computed_tokens)
+        child.status = SeqStatus.RUNNING
+        self._forced[child_id] = child
+        return page, slot
+
+    def _ready_to_force(self) -> None:
         assert self.is_driver and self.exec_world_size() == 1
         if self._pending is not None:
             self._drained_backlog.extend(self._drain_pending())
+
+    def _forced_rows(self, entries):
+        """Runs a forced step; the batch's logits and, of each logit row asked
+        for, its place among them."""
         bm = self.block_manager
         held = self._forced
-        if not entries:
-            for rid in end:
-                seq = held.pop(rid, None)
-                if seq is not None:
-                    bm.free(seq)
-                    if self.state_manager is not None:
-                        self.state_manager.free(seq)
-                    seq.status = SeqStatus.FINISHED
-            return torch.empty((0, self.cfg.model.vocab_size))
         prefill, chunks, decode = [], [], []
         need = 0
         for rid, tokens, _ in entries:
@@ -1066,26 +1128,10 @@ class LLMEngine:
             at = {r: r for r in range(len(decode))}
         else:
             at = {r: i for i, r in enumerate(rows)}
-        # an index that is a list would be copied to the GPU synchronously,
-        # and the host would stand still until this step is over
-        picked = [at[r] for r in asked]
-        if picked == list(range(logits.shape[0])):
-            out = logits.to(torch.float32, copy=True)
-        else:
-            out = logits.float()[self.runner._to_device(
-                {"rows": (picked, torch.long)})["rows"]]
         for seq in prefill + decode:
             seq.num_computed_tokens = seq.num_prompt_tokens
         self.num_prefilled_tokens += sum(chunks) + len(decode)
-        for rid in end:
-            seq = held.pop(rid, None)
-            if seq is None:
-                continue
-            bm.free(seq)
-            if self.state_manager is not None:
-                self.state_manager.free(seq)
-            seq.status = SeqStatus.FINISHED
-        return out
+        return logits, [at[r] for r in asked]
 
     # --------------------------------------------------------- TP workers
     def worker_loop(self) -> None:
@@ -1132,6 +1178,48 @@ class LLMEngine:
             self._ps.tp_broadcast_object({"kind": "stop"})
 
     # ------------------------------------------------------------ sync API
+    def next_request_id(self, prefix: str = "req") -> str:
+        return f"{prefix}-{next(self._req_counter)}"
+
+    def beam_search(
+        self,
+        prompts: List[List[int]],
+        beam_width: int = 4,
+        max_tokens: int = 128,
+        stop_token_ids=(),
+        length_penalty: float = 1.0,
+    ):
+        """Search with beams: for every prompt the ``beam_width`` best
+        hypotheses (engine/beam_search.py), best first by cumulative
+        log-probability over length ** length_penalty. ``stop_token_ids`` end
+        a hypothesis, as does max_model_len; without any, all have
+        ``max_tokens`` tokens. Searches run side by side as far as
+        max_num_seqs holds their beams, beside requests that are served, and
+        raise InsufficientBlocksError where the cache cannot hold them."""
+        from fusioninfer_amd.engine.beam_search import BeamSearcher
+
+        if self.exec_world_size() != 1:
+            raise ValueError("beam search unsupported with TP/PP")
+        limit = self.cfg.scheduler.max_model_len
+        seats = self.cfg.scheduler.max_num_seqs
+        if self.state_manager is not None:
+            seats = min(seats, self.state_manager.num_free())
+        if not 1 <= beam_width <= min(seats, ops.MOST_BEAMS):
+            raise ValueError(f"beam_width {beam_width} is not from 1 to "
+                             f"{min(seats, ops.MOST_BEAMS)}")
+        if max_tokens < 1:
+            raise ValueError("max_tokens is at least 1")
+        for p in prompts:
+            if not 1 <= len(p) < limit:
+                raise ValueError(f"prompt length {len(p)} leaves no room "
+                                 f"within max_model_len {limit}")
+        out = []
+        at_once = seats // beam_width
+        for i in range(0, len(prompts), at_once):
+            out += BeamSearcher(self, beam_width, max_tokens, stop_token_ids,
+                                length_penalty).run(prompts[i: i + at_once])
+        return out
+
     def generate(
         self,
         prompts: List[List[int]],

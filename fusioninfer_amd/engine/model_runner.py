@@ -160,6 +160,18 @@ class ModelRunner:
             for _ in range(self.model.num_local_layers)
         ]
 
+    def cache_tensors(self) -> Tuple[List[torch.Tensor], List[torch.Tensor]]:
+        """Every paged tensor, indexed by blocks, and every state tensor,
+        indexed by slots; one that layers share is listed once."""
+        pages, states = {}, {}
+        for cache in self.kv_caches:
+            named = (cache.items() if isinstance(cache, dict)
+                     else zip(("k", "v"), cache))
+            for name, t in named:
+                kind = pages if name in ("k", "v", "kv") else states
+                kind[t.data_ptr()] = t
+        return list(pages.values()), list(states.values())
+
     # ------------------------------------------------------------ inputs
     def _to_device(self, arrays):
         """A step's host arrays as device tensors, in one copy: dict of

@@ -60,7 +60,7 @@ class SamplingParams:
 
 
 class Sequence:
-    """One request = one sequence (no beam/parallel sampling in v1)."""
+    """One request = one sequence; a search with beams holds one per beam."""
 
     def __init__(self, seq_id: str, prompt_token_ids: List[int],
                  sampling: SamplingParams):
