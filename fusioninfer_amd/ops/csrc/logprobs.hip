@@ -345,8 +345,8 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
   for (int w = 0; w < kWaves; ++w) most = max(most, s_count[w]);
   if (most > kHeld) {
     // Many equal logits, or large ones in few of the groups. The bound becomes
-    // the k-th largest logit, and those that equal it are taken by index, in
-    // each wave up to the k-th.
+    // the k-th largest logit, and of those that equal it each wave takes, by
+    // index, as many as the larger ones leave of k: k in all at most.
     const auto above = [&](float v) {
       int count = 0;
 #pragma unroll
@@ -366,7 +366,8 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
     if (sizeof(A) == 4 && k > 1)
       bound = fmaxf(bound, value_of(few ? reached_by<0>(of_lane, k)
                                         : reached_by<0>(top, k)));
-    if (above(bound) >= k) {
+    int larger_ones = above(bound);
+    if (larger_ones >= k) {
       u32 lo = order_of(bound), hi = order_of(m);
       while (hi - lo > 1) {
         const u32 mid = lo + (hi - lo) / 2;
@@ -376,6 +377,7 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
           hi = mid;
       }
       bound = value_of(hi);
+      larger_ones = above(bound);
     }
     int equal = 0;
     held = 0;
@@ -392,7 +394,8 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
       }
 #pragma unroll
       for (int e = 0; e < L; ++e) {
-        const bool take = x[e] > bound || (x[e] == bound && rank < k);
+        const bool take =
+            x[e] > bound || (x[e] == bound && rank < k - larger_ones);
         rank += x[e] == bound;
         const u64 taken = __ballot(take);
         if (take)

@@ -77,6 +77,12 @@ def rows_of(kind, R, V, dtype, device, pad=0, start=0, seed=0):
         x[2::7, V - 1] = INF
     elif kind == "large":
         x = x * 1e30
+    elif kind == "clustered":  # large ones in few places of those at once
+        t = torch.arange(V) * dtype.itemsize // 16 % 64
+        x[:, t < 10] += 20
+    elif kind == "plateau":    # some above many equal ones
+        x = torch.where(torch.rand(R, V, generator=g) * V < 150, x.abs() + 9,
+                        -3.0)
     elif kind == "rising":
         x = torch.arange(V).float().repeat(R, 1) / V * 8
     wide = torch.full((R, V + pad + start), 77.0).to(dtype)
@@ -85,13 +91,13 @@ def rows_of(kind, R, V, dtype, device, pad=0, start=0, seed=0):
 
 
 KINDS = ["random", "steps", "equal", "zeros", "masked", "lowest", "gone",
-         "large", "rising"]
+         "large", "rising", "clustered", "plateau"]
 
 
 def scores_of(G, B, kind="", seed=1):
     g = torch.Generator().manual_seed(seed)
     s = -5 * torch.rand(G, B, generator=g)
-    if kind in ("steps", "equal", "zeros", "rising"):
+    if kind in ("steps", "equal", "zeros", "rising", "plateau"):
         s[:] = -1.25
     if kind == "gone":
         s[0, 0] = -INF
@@ -103,6 +109,7 @@ def scores_of(G, B, kind="", seed=1):
 @pytest.mark.parametrize("G,B,V,k", [
     (1, 1, 1, 1), (1, 1, 1, 3), (2, 3, 2, 8), (7, 4, 9, 8), (3, 5, 1000, 10),
     (2, 32, 5003, 64), (33, 2, 2050, 4), (1, 4, 16385, 8), (2, 3, 33001, 1),
+    (9, 8, 33001, 16), (9, 8, 33001, 230),
 ])
 @pytest.mark.parametrize("kind", KINDS)
 def test_beam_select(device, dtype, G, B, V, k, kind):
@@ -123,7 +130,7 @@ def test_beam_select(device, dtype, G, B, V, k, kind):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("R,V,k", [
     (1, 1, 0), (1, 1, 1), (3, 2, 2), (65, 9, 5), (4, 200, 200), (5, 1000, 20),
-    (2, 5003, 129), (2, 5003, 256), (257, 2050, 1), (3, 16385, 0), (2, 33001, 5),
+    (2, 5003, 129), (2, 5003, 256), (70, 16390, 256), (257, 2050, 1), (3, 16385, 0), (2, 33001, 5),
 ])
 @pytest.mark.parametrize("kind", KINDS)
 def test_top_logprobs(device, dtype, R, V, k, kind):
