@@ -33,6 +33,13 @@ constexpr float kLog2e = 1.44269504f;
 FI_DEV float logit_of(const float* p) { return *p; }
 FI_DEV float logit_of(const u16* p) { return bf16_to_f32(*p); }
 
+// 16 bytes of logits from anywhere, past the caches: of 2048 rows 93 us, 106
+// through them
+FI_DEV u32x4 read_once(const void* p) {
+  typedef u32x4 __attribute__((aligned(2))) Anywhere;
+  return __builtin_nontemporal_load(static_cast<const Anywhere*>(p));
+}
+
 // the logits of 16 bytes
 template <typename A>
 constexpr int kLanes = 16 / sizeof(A);
@@ -174,21 +181,23 @@ FI_DEV u32 reached_by(const u32 (&order)[N], int k) {
   return bound;
 }
 
-// A workgroup's chunk: VC groups of the logits that 16 bytes hold, NV of them a
-// thread. They are counted from the row's first logit wherever it lies, so that
+// A workgroup's chunk: NV groups of the logits that 16 bytes hold a thread. They
+// are counted from the row's first logit wherever it lies, so that
 // equal rows have equal sums; what the last group lacks counts as -inf.
 //
-// Four instructions per logit and the exponential's four cycles more are about
-// what memory leaves time for, so everything else is done per piece or per
-// thread: sums go on in 64 bits every piece (a sum that one term dominates
-// keeps the others), the bound is found from the threads' maxima, and the
-// logits of a piece are looked at only where its maximum reaches it.
+// About six instructions a bf16 logit, one of them the exponential of four
+// times the cycles, are what memory leaves time for (2048 rows of 152064: 87 us,
+// 7.2 TB/s), so everything else is done per piece or per thread: sums go on in
+// 64 bits every piece (a sum that one term dominates keeps the others), the
+// bound is found from the threads' maxima, and the logits of a piece are looked
+// at only where its maximum reaches it. Finding 16 of each row costs a fifth
+// more than none (512 rows of 151936: 32.5 us and 27).
 template <typename A, int NV>
 __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
     const A* __restrict__ logits, const int64_t stride, const int V,
-    const int chunks, const int VC, const int B, const int k,
-    ChunkSum* __restrict__ sums, u64* __restrict__ keys) {
-  constexpr int L = kLanes<A>;
+    const int chunks, const int B, const int k, ChunkSum* __restrict__ sums,
+    u64* __restrict__ keys) {
+  constexpr int L = kLanes<A>, VC = NV * kThreads;
   __shared__ float s_max[kThreads];
   __shared__ double s_sum[kWaves];
   __shared__ int s_count[kWaves];
@@ -205,10 +214,10 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
   u32x4 raw[NV];
   // a chunk's first logit, for pieces at 32-bit distances from it
   const A* from_first = row + static_cast<int64_t>(c) * VC * L;
-  if ((c * VC + NV * kThreads) * L <= V && VC == NV * kThreads) {
+  if ((c + 1) * VC * L <= V) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      __builtin_memcpy(&raw[i], from_first + i * kThreads * L + tid * L, 16);
+      raw[i] = read_once(from_first + i * kThreads * L + tid * L);
   } else {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -216,7 +225,7 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
       const u32 none = sizeof(A) == 4 ? 0xff800000u : 0xff80ff80u;
       raw[i] = u32x4{none, none, none, none};
       if (j < end && (j + 1) * L <= V)
-        __builtin_memcpy(&raw[i], row + static_cast<int64_t>(j) * L, 16);
+        raw[i] = read_once(row + static_cast<int64_t>(j) * L);
     }
     if (V % L && c == chunks - 1) {  // the last logits
       u32x4 tail = {0, 0, 0, 0};
@@ -571,7 +580,7 @@ FI_DEV void first_choices(const int lists, const int each, const int k,
   };
   take(first, 0);
   // places of all lists, and several a thread
-  const int step = (max(lists, 4 * T) + T - 1) / T * T;
+  const int step = (max(lists, kAhead * T) + T - 1) / T * T;
   for (int from = kAhead * T, n = 0; from < N; from += step) {
     if (from >= lists) {
       __syncthreads();
@@ -579,17 +588,16 @@ FI_DEV void first_choices(const int lists, const int each, const int k,
       ++n;
     }
     const int to = min(from + step, N);
-    for (int i0 = from; i0 < to; i0 += 4 * T) {
-      u64 next[4];
-      Choice more[4];
+    for (int i0 = from; i0 < to; i0 += kAhead * T) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int i = i0 + q * T + tid;
-        next[q] = i < to ? key(i) : 0;
+      for (int n = 0; n < kAhead; ++n) {
+        const int i = i0 + n * T + tid;
+        ahead_keys[n] = i < to ? key(i) : 0;
       }
 #pragma unroll
-      for (int q = 0; q < 4; ++q) more[q] = choice(i0 + q * T + tid, next[q]);
-      take(more, n);
+      for (int n = 0; n < kAhead; ++n)
+        first[n] = choice(i0 + n * T + tid, ahead_keys[n]);
+      take(first, n);
     }
   }
   __syncthreads();
@@ -755,9 +763,9 @@ __global__ __launch_bounds__(WAVES * kWaveSize) void top_join_kernel(
   }
 }
 
-// How a call is cut: NV pieces of 16 bytes a thread, VC a chunk.
+// How a call is cut: pieces of 16 bytes a thread, chunks a row.
 struct Cut {
-  int nv, chunks, vc;
+  int nv, chunks;
 };
 
 // Chunks as large as registers hold, 8 pieces a thread, leave the least to
@@ -768,12 +776,11 @@ struct Cut {
 Cut cut_of(int64_t R, int V, int size) {
   const int lanes = 16 / size;
   const int pieces = (V + lanes - 1) / lanes;
-  Cut cut{8, 0, 0};
+  Cut cut{8, 0};
   for (;; cut.nv /= 2) {
     cut.chunks = (pieces + cut.nv * kThreads - 1) / (cut.nv * kThreads);
     if (cut.nv == 1 || R * cut.chunks >= 64) break;
   }
-  cut.vc = cut.nv * kThreads;
   return cut;
 }
 
@@ -794,8 +801,7 @@ static Cut launch_logit_chunks(const A* logits, int64_t stride, int64_t R,
   const dim3 grid(R * cut.chunks);
 #define FI_CHUNKS(NV)                                                      \
   hipLaunchKernelGGL((logit_chunks_kernel<A, NV>), grid, dim3(kThreads), 0, \
-                     stream, logits, stride, V, cut.chunks, cut.vc, B, k,    \
-                     sums, keys)
+                     stream, logits, stride, V, cut.chunks, B, k, sums, keys)
   if (cut.nv == 8)
     FI_CHUNKS(8);
   else if (cut.nv == 4)
