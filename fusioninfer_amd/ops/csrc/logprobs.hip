@@ -505,7 +505,7 @@ FI_DEV RowSum join_sums(const ChunkSum* sums, int chunks, int lanes) {
 
 // The first k of the choices that `lists` lists hold, `each` of them in order:
 // key(i) is that of place i / lists of list i % lists, 0 beyond a list's end,
-// and choice(i, key) the choice. To put(place, choice); places that no choice
+// and choice(list, key) the choice. To put(place, choice); places that no choice
 // fills get one of score 0.
 //
 // A thread reads its first kAhead keys at once, before sums() joins the rows'
@@ -524,22 +524,36 @@ FI_DEV void first_choices(const int lists, const int each, const int k,
   __shared__ int s_beam[kTaken];
   const int tid = threadIdx.x, lane = tid % kWaveSize;
   const int N = lists * each;
-  u64 ahead_keys[kAhead];
+  u64 keys[kAhead];
+  const auto read = [&](int from) {
 #pragma unroll
-  for (int n = 0; n < kAhead; ++n)
-    ahead_keys[n] = tid + n * T < N ? key(tid + n * T) : 0;
+    for (int n = 0; n < kAhead; ++n) {
+      const int i = from + n * T + tid;
+      keys[n] = i < N ? key(i) : 0;
+    }
+  };
+  read(0);
   for (int i = tid; i < kTaken; i += T) s_score[i] = 0;
   if (tid < 2) s_reached[tid] = 0;
   if (tid == 0) s_count = 0;
   sums();
-  Choice first[kAhead];
+  // the lists of keys T apart
+  int list = tid % lists;
+  const int hop = T % lists;
+  Choice got[kAhead];
   u64 top = 0;
+  const auto weigh = [&](int from) {
 #pragma unroll
-  for (int n = 0; n < kAhead; ++n) {
-    first[n] = {0, 0, 0};
-    if (n * T < N) first[n] = choice(tid + n * T, ahead_keys[n]);
-    top = larger(top, first[n].score);
-  }
+    for (int n = 0; n < kAhead; ++n) {
+      got[n] = {0, 0, 0};
+      if (from + n * T < N) got[n] = choice(list, keys[n]);
+      list += hop;
+      if (list >= lists) list -= lists;
+    }
+  };
+  weigh(0);
+#pragma unroll
+  for (int n = 0; n < kAhead; ++n) top = larger(top, got[n].score);
   s_top[tid] = static_cast<u32>(top >> 32);
   __syncthreads();
   u32 tops[WAVES], of_lane[1] = {0};
@@ -552,13 +566,12 @@ FI_DEV void first_choices(const int lists, const int each, const int k,
   const u64 bound = larger<u64>(
       static_cast<u64>(k <= 32 ? reached_by<10>(of_lane, k)
                                : reached_by<10>(tops, k)) << 32, 1);
-  const auto take = [&](const auto& of, int step) {
-    constexpr int M = sizeof(of) / sizeof(Choice);
-    u64 reach[M];
+  const auto take = [&](int step) {
+    u64 reach[kAhead];
     int count = 0, at = 0;
 #pragma unroll
-    for (int n = 0; n < M; ++n) {
-      reach[n] = __ballot(of[n].score >= bound);
+    for (int n = 0; n < kAhead; ++n) {
+      reach[n] = __ballot(got[n].score >= bound);
       count += __popcll(reach[n]);
     }
     if (!count) return;
@@ -568,49 +581,54 @@ FI_DEV void first_choices(const int lists, const int each, const int k,
     }
     at = __builtin_amdgcn_readfirstlane(at);
 #pragma unroll
-    for (int n = 0; n < M; ++n) {
+    for (int n = 0; n < kAhead; ++n) {
       const int to = at + __popcll(reach[n] & ((1ull << lane) - 1));
-      if (of[n].score >= bound && to < kTaken) {
-        s_score[to] = of[n].score;
-        s_key[to] = of[n].key;
-        s_beam[to] = of[n].beam;
+      if (got[n].score >= bound && to < kTaken) {
+        s_score[to] = got[n].score;
+        s_key[to] = got[n].key;
+        s_beam[to] = got[n].beam;
       }
       at += __popcll(reach[n]);
     }
   };
-  take(first, 0);
-  // places of all lists, and several a thread
-  const int step = (max(lists, kAhead * T) + T - 1) / T * T;
-  for (int from = kAhead * T, n = 0; from < N; from += step) {
-    if (from >= lists) {
+  take(0);
+  // as many rounds as hold a place of all lists make a step
+  const int rounds = (lists + kAhead * T - 1) / (kAhead * T);
+  for (int n = 1; n * kAhead * T < N; ++n) {
+    const int step = n / rounds;
+    if (n % rounds == 0) {
       __syncthreads();
-      if (s_reached[n % 2] != n + 1) break;
-      ++n;
+      if (s_reached[(step - 1) % 2] != step) break;
     }
-    const int to = min(from + step, N);
-    for (int i0 = from; i0 < to; i0 += kAhead * T) {
-#pragma unroll
-      for (int n = 0; n < kAhead; ++n) {
-        const int i = i0 + n * T + tid;
-        ahead_keys[n] = i < to ? key(i) : 0;
-      }
-#pragma unroll
-      for (int n = 0; n < kAhead; ++n)
-        first[n] = choice(i0 + n * T + tid, ahead_keys[n]);
-      take(first, n);
-    }
+    read(n * kAhead * T);
+    weigh(n * kAhead * T);
+    take(step);
   }
   __syncthreads();
   const int all = s_count;
   if (all <= kTaken) {
     for (int i = tid; i < all; i += T) {
       const Choice mine{s_score[i], s_key[i], s_beam[i]};
-      int place = ahead_of(s_score, all, mine.score);
-      // itself, and now and then another with its score
-      if (ahead_of(s_score, all, mine.score - 1) != place + 1)
-        for (int j = 0; j < all; ++j)
-          place += s_score[j] == mine.score &&
-                   ahead({mine.score, s_key[j], s_beam[j]}, mine);
+      int place = 0, equal = 0;
+      for (int j = 0; j < all; j += kAtOnce) {
+#pragma unroll
+        for (int q = 0; q < kAtOnce; ++q) {
+          place += s_score[j + q] > mine.score;
+          equal += s_score[j + q] == mine.score;
+        }
+      }
+      if (equal > 1)  // equal logits of a beam, often
+        for (int j = 0; j < all; j += kAtOnce) {
+#pragma unroll
+          for (int q = 0; q < kAtOnce; ++q) {
+            // read without a question, else each read is a branch of its own
+            const u64 score = s_score[j + q], key = s_key[j + q];
+            const int beam = s_beam[j + q];
+            const bool first = (beam < mine.beam) |
+                               ((beam == mine.beam) & (key > mine.key));
+            place += (score == mine.score) & first;
+          }
+        }
       if (place < k) put(place, mine);
     }
     for (int i = all + tid; i < k; i += T) put(i, Choice{0, 0, 0});
@@ -622,7 +640,7 @@ FI_DEV void first_choices(const int lists, const int each, const int k,
     Choice best{0, 0, 0};
     if (last.score)
       for (int i = tid; i < N; i += T) {
-        const Choice c = choice(i, key(i));
+        const Choice c = choice(i % lists, key(i));
         if (c.score && ahead(last, c) && ahead(c, best)) best = c;
       }
     best = over_wave(best, [](const Choice& a, const Choice& b) {
@@ -679,8 +697,7 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(
         }
         __syncthreads();
       },
-      [&](int i, u64 key) -> Choice {
-        const int list = i % lists;
+      [&](int list, u64 key) -> Choice {
         const int b = quick ? __umulhi(list, by_chunks) : list / chunks;
         const double c = s_score[b];
         if (!key || !finite(c)) return {0, 0, 0};
