@@ -889,9 +889,9 @@ class LLMEngine:
         logits_rows covering every prompt position of requesting
         sequences; fill seq.prompt_logprobs (index 0 and prefix-cached
         positions are None) and return the standard sampling-row subset
-        in the engine's expected order. Rows are taken in slices: where a
-        slice's log-softmax has to be formed, it is never that of a full
-        8k-token admission."""
+        in the engine's expected order. Where a log-softmax has to be formed,
+        rows are taken in slices, so that a full 8k-token admission never
+        materializes a [T, V] fp32."""
         rows = payload["logits_rows"]
         pos_of = {r: i for i, r in enumerate(rows)}
         cu = payload["cu"]
@@ -912,11 +912,13 @@ class LLMEngine:
             # none after it
             first = pos_of[cu[j]] if n else 0
             n = min(n, seq.num_prompt_tokens - C - 1)
-            for lo in range(0, n, 256):
-                hi = min(lo + 256, n)
+            k = max(int(k), 0)
+            per = (max(n, 1) if logits_f.is_cuda and k <= ops.MOST_CHOICES
+                   else 256)
+            for lo in range(0, n, per):
+                hi = min(lo + per, n)
                 seq.prompt_logprobs.extend(self._logprob_entries(
-                    logits_f[first + lo: first + hi],
-                    [max(int(k), 0)] * (hi - lo),
+                    logits_f[first + lo: first + hi], [k] * (hi - lo),
                     toks[C + lo + 1: C + hi + 1]))
         pf_rows = [
             cu[j + 1] - 1 for j, smp in enumerate(payload["sample"]) if smp

@@ -83,6 +83,8 @@ def rows_of(kind, R, V, dtype, device, pad=0, start=0, seed=0):
     elif kind == "plateau":    # some above many equal ones
         x = torch.where(torch.rand(R, V, generator=g) * V < 150, x.abs() + 9,
                         -3.0)
+    elif kind == "tiny":       # below the normal numbers, still in order
+        x = x * 1e-40
     elif kind == "rising":
         x = torch.arange(V).float().repeat(R, 1) / V * 8
     wide = torch.full((R, V + pad + start), 77.0).to(dtype)
@@ -91,13 +93,13 @@ def rows_of(kind, R, V, dtype, device, pad=0, start=0, seed=0):
 
 
 KINDS = ["random", "steps", "equal", "zeros", "masked", "lowest", "gone",
-         "large", "rising", "clustered", "plateau"]
+         "large", "rising", "clustered", "plateau", "tiny"]
 
 
 def scores_of(G, B, kind="", seed=1):
     g = torch.Generator().manual_seed(seed)
     s = -5 * torch.rand(G, B, generator=g)
-    if kind in ("steps", "equal", "zeros", "rising", "plateau"):
+    if kind in ("steps", "equal", "zeros", "rising", "plateau", "tiny"):
         s[:] = -1.25
     if kind == "gone":
         s[0, 0] = -INF
