@@ -148,10 +148,10 @@ template void launch_kv_block_copy<false>(u16*, u16*, u16*, const int*, int,
 // with an id outside the tensor are passed over.
 //
 // What is written is not read again by this launch: stored past the caches it
-// takes 36 us for 239 MB of states and 117 us for 805 MB of whole e4m3 pages,
+// takes 36 us for 239 MB of states and 116 us for 805 MB of whole e4m3 pages,
 // 42 and 128 through them; loads past the caches lose (40 and 140), as beams
 // that go on from the same page read it again. 320 pages of 72 tensors, half
-// full, 802 MB: 157 us, 5.1 TB/s, where a copy of 2 GiB reaches 5.0.
+// full, 802 MB: 154 us, 5.2 TB/s, where a copy of 2 GiB reaches 5.0.
 __global__ __launch_bounds__(256) void copy_blocks_kernel(
     const BlockTensors tensors, const int* __restrict__ src,
     const int* __restrict__ dst, const int* __restrict__ tokens,

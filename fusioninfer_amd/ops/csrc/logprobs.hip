@@ -33,7 +33,7 @@ constexpr float kLog2e = 1.44269504f;
 FI_DEV float logit_of(const float* p) { return *p; }
 FI_DEV float logit_of(const u16* p) { return bf16_to_f32(*p); }
 
-// 16 bytes of logits from anywhere, past the caches: of 2048 rows 93 us, 106
+// 16 bytes of logits from anywhere, past the caches: 2048 rows 94 us a call, 106
 // through them
 FI_DEV u32x4 read_once(const void* p) {
   typedef u32x4 __attribute__((aligned(2))) Anywhere;
@@ -186,12 +186,12 @@ FI_DEV u32 reached_by(const u32 (&order)[N], int k) {
 // equal rows have equal sums; what the last group lacks counts as -inf.
 //
 // About six instructions a bf16 logit, one of them the exponential of four
-// times the cycles, are what memory leaves time for (2048 rows of 152064: 87 us,
-// 7.2 TB/s), so everything else is done per piece or per thread: sums go on in
-// 64 bits every piece (a sum that one term dominates keeps the others), the
-// bound is found from the threads' maxima, and the logits of a piece are looked
-// at only where its maximum reaches it. Finding 16 of each row costs a fifth
-// more than none (512 rows of 151936: 32.5 us and 27).
+// times the cycles, are what memory leaves time for (2048 rows of 152064: 94 us
+// a call, 6.6 TB/s), so everything else is done per piece or per thread: sums go
+// on in 64 bits every piece (a sum that one term dominates keeps the others),
+// the bound is found from the threads' maxima, and the logits of a piece are
+// looked at only where its maximum reaches it. Finding 16 of each row costs a
+// fifth more than none (512 rows of 151936: 32.5 us and 27).
 template <typename A, int NV>
 __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
     const A* __restrict__ logits, const int64_t stride, const int V,
@@ -786,10 +786,10 @@ struct Cut {
 };
 
 // Chunks as large as registers hold, 8 pieces a thread, leave the least to
-// join; halved until 64 workgroups share the call. One search of 4 beams over
-// 151936 tokens 12.3 us so, 14.1 by 256 to 2048 workgroups, which read faster
-// but have twice as much to join; 64 searches of 8 47 us, 49 with 4 pieces. Sixteen
-// pieces are no faster.
+// join; halved until 64 workgroups share the call. With the joins of that step
+// one search of 4 beams over 151936 tokens took 12.3 us so, 14.1 by 256 to 2048
+// workgroups, which read faster but leave twice as much to join; 64 searches of
+// 8 beams 47 us, 49 with 4 pieces. Sixteen pieces are no faster.
 Cut cut_of(int64_t R, int V, int size) {
   const int lanes = 16 / size;
   const int pieces = (V + lanes - 1) / lanes;
