@@ -9,10 +9,9 @@ of the recurrent state, all of a step's copies in one launch for pages and one
 for states. Beams without a continuation give their blocks back first, so that
 a step needs no more blocks than its beams hold.
 
-Capability parity: the beam search of the engine that the reference delegates
-to its vLLM containers (a continuation that ends with a stop token is a
-finished hypothesis; final order by cumulative log-probability over
-length ** length_penalty).
+A continuation that ends with a stop token is a finished hypothesis if it ranks
+before the last beam kept; hypotheses are ordered by cumulative log-probability
+over length ** length_penalty.
 """
 
 from __future__ import annotations
