@@ -1203,11 +1203,15 @@ def moe_combine_norm(y, pos, w, residual, weight, eps: float):
 
 MOST_CHOICES = 256  # of one row or search
 MOST_BEAMS = 256    # of one search
+MOST_CHUNKS = 5120  # of 8192 tokens, of all beams of a search
 
 
-def _check_rows(logits, k: int, most: int) -> None:
+def _check_rows(logits, k: int, most: int, beams: int = 1) -> None:
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError("logits are rows of at least one token")
+    if beams * -(-logits.shape[1] // 8192) > MOST_CHUNKS:
+        raise ValueError(f"{beams} beams over {logits.shape[1]} tokens are "
+                         "too many in one search")
     if logits.dtype not in (torch.float32, torch.bfloat16):
         raise ValueError("logits are float32 or bfloat16")
     if not 0 <= k <= most:
@@ -1231,7 +1235,7 @@ def top_logprobs(logits: torch.Tensor, k: int,
     ordered by logit, equal ones by token, those at -inf last. A row without a
     distribution (a NaN or +inf in it, or -inf throughout) is NaN, its tokens
     0 to k-1. A given token outside [0, V) has -inf. k: 0 to V, at most
-    MOST_CHOICES."""
+    MOST_CHOICES; V: up to some 40 million."""
     if logits.is_cuda:
         _require_native()
         return TopLogprobs(*_C.top_logprobs(logits, k, token_ids))
@@ -1263,13 +1267,16 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor,
     by logit, then by token. A token at -inf is no continuation, nor is any
     of a beam whose score is not finite (-inf: a beam that has ended or not
     begun) or whose row has no distribution (a NaN or +inf in it). Places
-    without a continuation hold score -inf, beam -1 and token -1. B: up to
-    MOST_BEAMS. k: 1 to MOST_CHOICES; twice the number of beams leaves enough of them where up
-    to one continuation of each beam ends it."""
+    without a continuation hold score -inf, beam -1 and token -1.
+
+    B: up to MOST_BEAMS, and B times V up to some 40 million. k: 1 to
+    MOST_CHOICES; twice the number of beams leaves enough of them where up to
+    one continuation of each beam ends it."""
     if logits.is_cuda:
         _require_native()
         return BeamChoice(*_C.beam_select(logits, scores, k))
-    _check_rows(logits, k, MOST_CHOICES)
+    _check_rows(logits, k, MOST_CHOICES,
+                scores.shape[1] if scores.dim() == 2 else 1)
     if k < 1:
         raise ValueError("k is at least 1")
     if scores.dim() != 2 or scores.dtype != torch.float32 \

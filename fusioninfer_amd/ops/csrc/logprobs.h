@@ -8,6 +8,8 @@ namespace fi {
 
 constexpr int kMostChoices = 256;
 constexpr int kMostBeams = 256;  // of one search
+// chunks of a search's rows, of 8192 logits or more where they are many
+constexpr int kMostLists = 5120;
 
 // bytes of workspace of a call on R rows of V tokens of `size` bytes
 int64_t logit_workspace(int64_t R, int V, int k, int size);

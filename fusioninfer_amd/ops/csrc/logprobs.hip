@@ -506,23 +506,27 @@ FI_DEV RowSum join_sums(const ChunkSum* sums, int chunks, int lanes) {
 // The first k of the choices that `lists` lists hold, `each` of them in order:
 // key(i) is that of place i / lists of list i % lists, 0 beyond a list's end,
 // and choice(list, key) the choice. To put(place, choice); places that no choice
-// fills get one of score 0.
+// fills get one of score 0. near(score, best) orders scores in 32 bits.
 //
 // A thread reads its first kAhead keys at once, before sums() joins the rows'
-// sums: a join is one workgroup's chain of waits. The bound is found from the
-// threads' best ones, beginning with the lists' first. Further places are read
-// in turn until one of all lists holds nothing that reaches it.
+// sums: a join is one workgroup's chain of waits. The bound is the k-th largest
+// of 64 maxima of those, beyond k = 32 of all of them. Further places are read in
+// turn until one of all lists holds nothing that reaches it. Where more reach it
+// than LDS holds (equal ones), the lists are merged, a choice a round.
 constexpr int kAhead = 8;
-template <int WAVES, class Key, class Sums, class Of, class Put>
+constexpr int kLastBit = 8;  // of the bound: fifteen bits of mantissa
+template <int WAVES, class Key, class Sums, class Of, class Near, class Put>
 FI_DEV void first_choices(const int lists, const int each, const int k,
-                          Key key, Sums sums, Of choice, Put put) {
+                          Key key, Sums sums, Of choice, Near near, Put put) {
   constexpr int T = WAVES * kWaveSize, kTaken = 2 * T;
-  __shared__ u32 s_top[T];
-  __shared__ int s_count, s_reached[2];
+  __shared__ u64 s_top[T];
+  __shared__ int s_count, s_reached[2], s_full[2], s_votes[2][WAVES];
   __shared__ __attribute__((aligned(16))) u64 s_score[kTaken];
   __shared__ u64 s_key[kTaken];
   __shared__ int s_beam[kTaken];
+  __shared__ u16 s_place[WAVES > 1 ? kMostLists : kAhead * T];
   const int tid = threadIdx.x, lane = tid % kWaveSize;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWaveSize);
   const int N = lists * each;
   u64 keys[kAhead];
   const auto read = [&](int from) {
@@ -534,14 +538,13 @@ FI_DEV void first_choices(const int lists, const int each, const int k,
   };
   read(0);
   for (int i = tid; i < kTaken; i += T) s_score[i] = 0;
-  if (tid < 2) s_reached[tid] = 0;
+  if (tid < 2) s_reached[tid] = s_full[tid] = 0;
   if (tid == 0) s_count = 0;
   sums();
   // the lists of keys T apart
   int list = tid % lists;
   const int hop = T % lists;
   Choice got[kAhead];
-  u64 top = 0;
   const auto weigh = [&](int from) {
 #pragma unroll
     for (int n = 0; n < kAhead; ++n) {
@@ -552,38 +555,60 @@ FI_DEV void first_choices(const int lists, const int each, const int k,
     }
   };
   weigh(0);
+  u64 top = 0;
 #pragma unroll
   for (int n = 0; n < kAhead; ++n) top = larger(top, got[n].score);
-  s_top[tid] = static_cast<u32>(top >> 32);
+  s_top[tid] = top;
   __syncthreads();
-  u32 tops[WAVES], of_lane[1] = {0};
+  top = 0;
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    tops[w] = s_top[w * kWaveSize + lane];
-    of_lane[0] = larger(of_lane[0], tops[w]);
+  for (int w = 0; w < WAVES; ++w)
+    top = larger(top, s_top[w * kWaveSize + lane]);
+  const u64 best = over_wave(top, larger<u64>);
+  const auto order = [&](u64 score) { return score ? near(score, best) : 0; };
+  u32 of_got[kAhead], bound = 0;
+#pragma unroll
+  for (int n = 0; n < kAhead; ++n) of_got[n] = order(got[n].score);
+  if (k <= 32) {
+    const u32 of_lane[1] = {order(top)};
+    bound = reached_by<kLastBit>(of_lane, k);
+  } else {
+    for (int bit = 31; bit >= kLastBit; --bit) {
+      const u32 next = bound | 1u << bit;
+      int count = 0;
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n)
+        count += __popcll(__ballot(of_got[n] >= next));
+      if constexpr (WAVES > 1) {
+        if (lane == 0) s_votes[bit % 2][wave] = count;
+        __syncthreads();
+        count = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) count += s_votes[bit % 2][w];
+      }
+      if (count >= k) bound = next;
+    }
   }
-  // ten bits of mantissa of a score in 64 bits, thirteen of a logit
-  const u64 bound = larger<u64>(
-      static_cast<u64>(k <= 32 ? reached_by<10>(of_lane, k)
-                               : reached_by<10>(tops, k)) << 32, 1);
+  bound = larger(bound, 1u);
   const auto take = [&](int step) {
     u64 reach[kAhead];
     int count = 0, at = 0;
 #pragma unroll
     for (int n = 0; n < kAhead; ++n) {
-      reach[n] = __ballot(got[n].score >= bound);
+      reach[n] = __ballot(of_got[n] >= bound);
       count += __popcll(reach[n]);
     }
     if (!count) return;
     if (lane == 0) {
       at = atomicAdd(&s_count, count);
       s_reached[step % 2] = step + 1;
+      if (at + count > kTaken) s_full[step % 2] = step + 1;
     }
     at = __builtin_amdgcn_readfirstlane(at);
 #pragma unroll
     for (int n = 0; n < kAhead; ++n) {
       const int to = at + __popcll(reach[n] & ((1ull << lane) - 1));
-      if (got[n].score >= bound && to < kTaken) {
+      if (of_got[n] >= bound && to < kTaken) {
         s_score[to] = got[n].score;
         s_key[to] = got[n].key;
         s_beam[to] = got[n].beam;
@@ -597,11 +622,15 @@ FI_DEV void first_choices(const int lists, const int each, const int k,
   for (int n = 1; n * kAhead * T < N; ++n) {
     const int step = n / rounds;
     if (n % rounds == 0) {
+      // what the others set from here on is the next step's
       __syncthreads();
-      if (s_reached[(step - 1) % 2] != step) break;
+      const int last = (step - 1) % 2;
+      if (s_reached[last] != step || s_full[last] == step) break;
     }
     read(n * kAhead * T);
     weigh(n * kAhead * T);
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) of_got[q] = order(got[q].score);
     take(step);
   }
   __syncthreads();
@@ -634,31 +663,44 @@ FI_DEV void first_choices(const int lists, const int each, const int k,
     for (int i = all + tid; i < k; i += T) put(i, Choice{0, 0, 0});
     return;
   }
-  // more equal ones than fit: a round of the workgroup each
-  Choice last{~0ull, 0, -1};
-  for (int n = 0; n < k; ++n) {
-    Choice best{0, 0, 0};
-    if (last.score)
-      for (int i = tid; i < N; i += T) {
-        const Choice c = choice(i % lists, key(i));
-        if (c.score && ahead(last, c) && ahead(c, best)) best = c;
+  // A thread's lists are T apart; it keeps the best of their heads.
+  Choice head{0, 0, 0};
+  int of = 0;
+  const auto find = [&] {
+    head = {0, 0, 0};
+    for (int v = tid; v < lists; v += T) {
+      const int at = s_place[v];
+      if (at == each) continue;
+      const Choice c = choice(v, key(at * lists + v));
+      if (c.score && ahead(c, head)) {
+        head = c;
+        of = v;
       }
-    best = over_wave(best, [](const Choice& a, const Choice& b) {
+    }
+  };
+  __syncthreads();
+  for (int v = tid; v < lists; v += T) s_place[v] = 0;
+  find();
+  for (int n = 0; n < k; ++n) {
+    Choice first = over_wave(head, [](const Choice& a, const Choice& b) {
       return ahead(b, a) ? b : a;
     });
     __syncthreads();
     if (lane == 0) {
-      s_score[tid / kWaveSize] = best.score;
-      s_key[tid / kWaveSize] = best.key;
-      s_beam[tid / kWaveSize] = best.beam;
+      s_top[wave] = first.key;
+      s_score[wave] = first.score;
+      s_beam[wave] = first.beam;
     }
     __syncthreads();
     for (int w = 0; w < WAVES; ++w) {
-      const Choice of{s_score[w], s_key[w], s_beam[w]};
-      if (ahead(of, best)) best = of;
+      const Choice c{s_score[w], s_top[w], s_beam[w]};
+      if (ahead(c, first)) first = c;
     }
-    if (tid == 0) put(n, best);
-    last = best;
+    if (tid == 0) put(n, first);
+    if (first.score && first.key == head.key && first.beam == head.beam) {
+      ++s_place[of];
+      find();
+    }
   }
 }
 
@@ -702,6 +744,11 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(
         const double c = s_score[b];
         if (!key || !finite(c)) return {0, 0, 0};
         return {score_order(c + s_row[b].of(value_of(key >> 32))), key, b};
+      },
+      // by how far it is from the best, whatever the scores have come to
+      [](u64 score, u64 best) {
+        return order_of(
+            static_cast<float>(score_value(score) - score_value(best)));
       },
       [&](int i, const Choice& c) {
         const bool some = c.score != 0;
@@ -753,6 +800,7 @@ __global__ __launch_bounds__(WAVES * kWaveSize) void top_join_kernel(
       [&](int, u64 key) -> Choice {
         return {z.alive() ? key : 0, key, 0};
       },
+      [](u64 key, u64) { return static_cast<u32>(key >> 32); },
       [&](int i, const Choice& c) {
         if (c.score) {
           out_lp[i] = z.of(value_of(c.key >> 32));

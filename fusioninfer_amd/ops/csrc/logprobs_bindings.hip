@@ -46,6 +46,11 @@ at::Tensor rows_of(const at::Tensor& t) {
   return t.contiguous();
 }
 
+void check_search(int64_t beams, int64_t tokens) {
+  CHECK_THAT(beams * ((tokens + 8191) / 8192) <= fi::kMostLists, beams,
+             " beams over ", tokens, " tokens are too many in one search");
+}
+
 // scores [G, k], parents [G, k], tokens [G, k]
 std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_select(
     const at::Tensor& of, const at::Tensor& scores, int64_t k) {
@@ -59,9 +64,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_select(
   const int64_t G = scores.size(0), B = scores.size(1);
   CHECK_THAT(G * B == logits.size(0) && B >= 1 && B <= fi::kMostBeams,
              logits.size(0), " rows of logits for [", G, ", ", B, "] beams");
-  // the choices of a search are counted in 32 bits
-  CHECK_THAT((logits.size(1) / 1024 + 1) * B * k < (1ll << 31),
-             "too many logits and choices in one search");
+  check_search(B, logits.size(1));
   const Guard guard(logits.device());
   const auto f32 = logits.options().dtype(at::kFloat);
   const auto i32 = logits.options().dtype(at::kInt);
@@ -95,6 +98,7 @@ std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>> top_logprobs(
   const int64_t R = logits.size(0);
   const int64_t most = std::min<int64_t>(fi::kMostChoices, logits.size(1));
   CHECK_THAT(k >= 0 && k <= most, "k is ", k, ", not from 0 to ", most);
+  check_search(1, logits.size(1));
   c10::optional<at::Tensor> given;
   if (token_ids) {
     CHECK_THAT(token_ids->device() == logits.device() &&

@@ -183,6 +183,19 @@ def test_most_choices_of_one_row(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("k", [8, 60])
+def test_long_beams(device, k):
+    """Scores far below what one token adds or takes."""
+    x = rows_of("random", 16, 2500, torch.bfloat16, device)
+    c = -30000 + scores_of(2, 8)
+    got = ops.beam_select(x, c.to(device), k)
+    s, p, t = beams64(x, c, k)
+    assert np.array_equal(got.parents.cpu().numpy(), p)
+    assert np.array_equal(got.tokens.cpu().numpy(), t)
+    near(got.scores, s, 2500)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_scores_cut_from_the_last_choice(device):
     """As a search goes on: the first B of its 2B candidates."""
     x = rows_of("random", 12, 501, torch.bfloat16, device)
@@ -227,6 +240,8 @@ def test_refusals(device):
         lambda: ops.beam_select(
             x.new_zeros(ops.MOST_BEAMS + 1, 3),
             x.new_zeros(1, ops.MOST_BEAMS + 1), 2),
+        lambda: ops.beam_select(
+            x.new_zeros(256, 1).expand(256, 163_841), x.new_zeros(1, 256), 2),
         lambda: ops.top_logprobs(x, 11),
         lambda: ops.top_logprobs(x, -1),
         lambda: ops.top_logprobs(x.double(), 2),
