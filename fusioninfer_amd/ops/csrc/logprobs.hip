@@ -18,6 +18,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "logprobs.h"
 
 namespace fi {
@@ -200,7 +202,7 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
   constexpr int L = kLanes<A>, VC = NV * kThreads;
   __shared__ float s_max[kThreads];
   __shared__ double s_sum[kWaves];
-  __shared__ int s_count[kWaves];
+  __shared__ int s_count[kWaves], s_votes[2][kWaves];
   __shared__ __attribute__((aligned(16))) u64 s_key[kWaves][kHeld + kAtOnce];
   const int tid = threadIdx.x, lane = tid % kWaveSize;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWaveSize);
@@ -257,22 +259,52 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
   }
   s_max[tid] = m;
   __syncthreads();
-  // Groups of four threads for small k, a sixteenth more values than k for 16 of
-  // 64 groups, two fifths for 32; then each thread is one.
-  u32 top[kWaves], of_lane[1] = {0};
+  // The groups: four threads each for small k (a sixteenth more values than k
+  // reach the bound for 16 of 64 groups, two fifths for 32), a thread each up to
+  // half of their number, then a piece each, whose votes the waves exchange.
+  float of_thread[kWaves];
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
-    const float v = s_max[w * kWaveSize + lane];
-    m = fmaxf(m, v);
-    top[w] = order_of(v);
-    of_lane[0] = larger(of_lane[0], top[w]);
+    of_thread[w] = s_max[w * kWaveSize + lane];
+    m = fmaxf(m, of_thread[w]);
   }
+  const float of_lane = m;
   m = wave_reduce_max(m);
-  const bool few = k <= 32;
+  const auto reached_by_pieces = [&](int last) {
+    u32 order[NV], reached = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) order[i] = order_of(piece[i]);
+    for (int bit = 31; bit >= last; --bit) {
+      const u32 next = reached | 1u << bit;
+      int count = 0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        count += __popcll(__ballot(order[i] >= next));
+      if (lane == 0) s_votes[bit % 2][wave] = count;
+      __syncthreads();
+      count = 0;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) count += s_votes[bit % 2][w];
+      if (count >= k) reached = next;
+    }
+    return reached;
+  };
+  const auto reached = [&](auto last) {
+    constexpr int kLast = decltype(last)::value;
+    if (k <= 32) {
+      const u32 order[1] = {order_of(of_lane)};
+      return reached_by<kLast>(order, k);
+    }
+    if (k > kThreads / 2) return reached_by_pieces(kLast);
+    u32 order[kWaves];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) order[w] = order_of(of_thread[w]);
+    return reached_by<kLast>(order, k);
+  };
   // sixteen bits of the order are a bf16 value's, and as near as 2^-7 to others
   float bound = m;
   if (k > 1) {
-    u32 order = few ? reached_by<16>(of_lane, k) : reached_by<16>(top, k);
+    u32 order = reached(std::integral_constant<int, 16>());
     if (sizeof(A) == 2 && !(order >> 31)) order |= 0xffffu;
     bound = value_of(order);
   }
@@ -373,8 +405,8 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
       return count;
     };
     if (sizeof(A) == 4 && k > 1)
-      bound = fmaxf(bound, value_of(few ? reached_by<0>(of_lane, k)
-                                        : reached_by<0>(top, k)));
+      bound = fmaxf(bound,
+                    value_of(reached(std::integral_constant<int, 0>())));
     int larger_ones = above(bound);
     if (larger_ones >= k) {
       u32 lo = order_of(bound), hi = order_of(m);
@@ -509,9 +541,9 @@ FI_DEV RowSum join_sums(const ChunkSum* sums, int chunks, int lanes) {
 // fills get one of score 0. near(score, best) orders scores in 32 bits.
 //
 // A thread reads its first kAhead keys at once, before sums() joins the rows'
-// sums: a join is one workgroup's chain of waits. The bound is the k-th largest
-// of 64 maxima of those, beyond k = 32 of all of them. Further places are read in
-// turn until one of all lists holds nothing that reaches it. Where more reach it
+// sums: a join is one workgroup's chain of waits. The bound comes from groups of
+// those as a chunk's does. Further places are read in turn until one of all lists
+// holds nothing that reaches it. Where more reach it
 // than LDS holds (equal ones), the lists are merged, a choice a round.
 constexpr int kAhead = 8;
 constexpr int kLastBit = 8;  // of the bound: fifteen bits of mantissa
@@ -561,9 +593,12 @@ FI_DEV void first_choices(const int lists, const int each, const int k,
   s_top[tid] = top;
   __syncthreads();
   top = 0;
+  u64 tops[WAVES];
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w)
-    top = larger(top, s_top[w * kWaveSize + lane]);
+  for (int w = 0; w < WAVES; ++w) {
+    tops[w] = s_top[w * kWaveSize + lane];
+    top = larger(top, tops[w]);
+  }
   const u64 best = over_wave(top, larger<u64>);
   const auto order = [&](u64 score) { return score ? near(score, best) : 0; };
   u32 of_got[kAhead], bound = 0;
@@ -572,6 +607,11 @@ FI_DEV void first_choices(const int lists, const int each, const int k,
   if (k <= 32) {
     const u32 of_lane[1] = {order(top)};
     bound = reached_by<kLastBit>(of_lane, k);
+  } else if (k <= T / 2) {
+    u32 of_thread[WAVES];
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) of_thread[w] = order(tops[w]);
+    bound = reached_by<kLastBit>(of_thread, k);
   } else {
     for (int bit = 31; bit >= kLastBit; --bit) {
       const u32 next = bound | 1u << bit;
@@ -834,17 +874,20 @@ struct Cut {
 };
 
 // Chunks as large as registers hold, 8 pieces a thread, leave the least to
-// join; halved until 64 workgroups share the call. With the joins of that step
-// one search of 4 beams over 151936 tokens took 12.3 us so, 14.1 by 256 to 2048
-// workgroups, which read faster but leave twice as much to join; 64 searches of
-// 8 beams 47 us, 49 with 4 pieces. Sixteen pieces are no faster.
-Cut cut_of(int64_t R, int V, int size) {
+// join; halved until 64 workgroups share the call, as long as a chunk has four
+// times as many pieces as it gives keys (256 choices of one row 32 us, 142
+// without). With the joins of that step one search of 4 beams over 151936 tokens
+// took 12.3 us so, 14.1 by 256 to 2048 workgroups, which read faster but leave
+// twice as much to join; 64 searches of 8 beams 47 us, 49 with 4 pieces. Sixteen
+// pieces are no faster.
+Cut cut_of(int64_t R, int V, int k, int size) {
   const int lanes = 16 / size;
   const int pieces = (V + lanes - 1) / lanes;
   Cut cut{8, 0};
   for (;; cut.nv /= 2) {
     cut.chunks = (pieces + cut.nv * kThreads - 1) / (cut.nv * kThreads);
-    if (cut.nv == 1 || R * cut.chunks >= 64) break;
+    if (cut.nv == 1 || R * cut.chunks >= 64 || cut.nv * kThreads < 8 * k)
+      break;
   }
   return cut;
 }
@@ -852,7 +895,7 @@ Cut cut_of(int64_t R, int V, int size) {
 }  // namespace
 
 int64_t logit_workspace(int64_t R, int V, int k, int size) {
-  return R * cut_of(R, V, size).chunks *
+  return R * cut_of(R, V, k, size).chunks *
          static_cast<int64_t>(sizeof(ChunkSum) + k * sizeof(u64));
 }
 
@@ -860,7 +903,7 @@ template <typename A>
 static Cut launch_logit_chunks(const A* logits, int64_t stride, int64_t R,
                                int V, int B, int k, void* workspace,
                                hipStream_t stream) {
-  const Cut cut = cut_of(R, V, sizeof(A));
+  const Cut cut = cut_of(R, V, k, sizeof(A));
   ChunkSum* sums = static_cast<ChunkSum*>(workspace);
   u64* keys = reinterpret_cast<u64*>(sums + R * cut.chunks);
   const dim3 grid(R * cut.chunks);
