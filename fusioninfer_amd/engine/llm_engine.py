@@ -913,7 +913,7 @@ class LLMEngine:
             first = pos_of[cu[j]] if n else 0
             n = min(n, seq.num_prompt_tokens - C - 1)
             k = max(int(k), 0)
-            per = (max(n, 1) if logits_f.is_cuda and k <= ops.MOST_CHOICES
+            per = (8192 if logits_f.is_cuda and k <= ops.MOST_CHOICES
                    else 256)
             for lo in range(0, n, per):
                 hi = min(lo + per, n)
@@ -1197,7 +1197,10 @@ class LLMEngine:
         a hypothesis, as does max_model_len; without any, all have
         ``max_tokens`` tokens. Searches run side by side as far as
         max_num_seqs holds their beams, beside requests that are served, and
-        raise InsufficientBlocksError where the cache cannot hold them."""
+        raise InsufficientBlocksError where the cache cannot hold them. A step
+        looks at the ops.MOST_CHOICES best continuations of a search at most:
+        where so many of them end that fewer than ``beam_width`` are left, it
+        goes on with those."""
         from fusioninfer_amd.engine.beam_search import BeamSearcher
 
         if self.exec_world_size() != 1:

@@ -58,7 +58,8 @@ FI_DEV void unpack(const u32x4 raw, float (&x)[8], const u16*) {
 }
 
 // maximum of three; written out, as the compiler first maxes every operand with
-// itself for the sake of signaling NaNs, which leave no distribution anyway
+// itself for the sake of signaling NaNs: one makes the maximum NaN, which the next
+// fmaxf passes over, and leaves no distribution anyway
 FI_DEV float max3(float a, float b, float c) {
   float v = 0.f;
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -439,12 +440,15 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
             x[e] > bound || (x[e] == bound && rank < k - larger_ones);
         rank += x[e] == bound;
         const u64 taken = __ballot(take);
-        if (take)
-          s_key[wave][held + __popcll(taken & below)] =
-              key_of(x[e], (first + i * kThreads) * L + e);
+        const int at = held + __popcll(taken & below);
+        if (take && at < kHeld)
+          s_key[wave][at] = key_of(x[e], (first + i * kThreads) * L + e);
         held += __popcll(taken);
       }
     }
+    // more only where a signaling NaN hid its piece's logits from the maximum:
+    // the row has no distribution
+    held = min(held, kHeld);
     if (lane < kAtOnce) s_key[wave][held + lane] = 0;
     __syncthreads();
     if (lane == 0) s_count[wave] = held;

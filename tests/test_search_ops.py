@@ -183,6 +183,33 @@ def test_most_choices_of_one_row(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype,integer,nan", [
+    (torch.float32, torch.int32, 0x7f810000),
+    (torch.bfloat16, torch.int16, 0x7f81)])
+@pytest.mark.parametrize("k", [1, 20, 100, 230])
+def test_signaling_nans_before_many_large_logits(device, dtype, integer, nan, k):
+    """They may hide the logits beside them from a maximum, so that more than
+    k are larger than what is found to be the largest."""
+    x = rows_of("random", 6, 20000, dtype, "cpu", pad=3, start=1)
+    want = ops.top_logprobs(x.to(device), k)
+    c = scores_of(2, 3)
+    c[1, 2] = -INF
+    beams = ops.beam_select(x.to(device), c.to(device), k)
+    pieces = x[5, :20000].unfold(0, 16 // dtype.itemsize, 16 // dtype.itemsize)
+    pieces[::3] += 50
+    pieces[::3, -1] = torch.tensor([nan], dtype=integer).view(dtype)
+    assert torch.isnan(x[5]).any()
+    got = ops.top_logprobs(x.to(device), k)
+    assert torch.equal(got.logprobs[:5], want.logprobs[:5])
+    assert torch.equal(got.ids[:5], want.ids[:5])
+    assert torch.isnan(got.logprobs[5]).all()
+    assert got.ids[5].tolist() == list(range(k))
+    c[1, 2] = -1.0
+    for a, b in zip(ops.beam_select(x.to(device), c.to(device), k), beams):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("k", [8, 60])
 def test_long_beams(device, k):
     """Scores far below what one token adds or takes."""
