@@ -86,7 +86,7 @@ FI_DEV int token_of(u64 key) {
 
 // The value of the lane 32, 16, 8, 4, 2 or 1 away, in a reduction that goes
 // through these steps in turn: 4 away by a rotation, which takes what repeats
-// every 8 lanes.
+// every 8 lanes. STEP 7: of the lane as far from the other end of 8.
 template <int STEP>
 FI_DEV u32 partner(u32 v) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -96,9 +96,12 @@ FI_DEV u32 partner(u32 v) {
                        : __builtin_amdgcn_permlane16_swap(v, v, false, false);
     return __lane_id() & STEP ? r[0] : r[1];
   } else {
-    // row_ror:8, row_ror:4, quad_perm [2,3,0,1] and [1,0,3,2]
-    constexpr int ctrl =
-        STEP == 8 ? 0x128 : STEP == 4 ? 0x124 : STEP == 2 ? 0x4E : 0xB1;
+    // row_ror:8, row_half_mirror, row_ror:4, quad_perm [2,3,0,1] and [1,0,3,2]
+    constexpr int ctrl = STEP == 8   ? 0x128
+                         : STEP == 7 ? 0x141
+                         : STEP == 4 ? 0x124
+                         : STEP == 2 ? 0x4E
+                                     : 0xB1;
     return __builtin_amdgcn_update_dpp(0, v, ctrl, 0xF, 0xF, true);
   }
 #else
@@ -509,17 +512,21 @@ struct RowSum {
   FI_DEV double of(float v) const { return (static_cast<double>(v) - m) - ln; }
 };
 
-// Joined by groups of 16, 32 or 64 lanes, whichever hold the chunks of a row
+// Joined by groups of 8, 16, 32 or 64 lanes, whichever hold the chunks of a row
 // (64 go round), in all of the group's lanes. Rows of sums begin at `sums`.
 FI_DEV int lanes_for(int chunks) {
-  return chunks <= 16 ? 16 : chunks <= 32 ? 32 : kWaveSize;
+  return chunks <= 8 ? 8 : chunks <= 16 ? 16 : chunks <= 32 ? 32 : kWaveSize;
 }
 template <class T, class Op>
 FI_DEV T over_lanes(T v, int lanes, Op op) {
   if (lanes > 32) v = op(v, partner<32>(v));
   if (lanes > 16) v = op(v, partner<16>(v));
-  v = op(v, partner<8>(v));
-  v = op(v, partner<4>(v));
+  if (lanes > 8) {
+    v = op(v, partner<8>(v));
+    v = op(v, partner<4>(v));
+  } else {
+    v = op(v, partner<7>(v));
+  }
   v = op(v, partner<2>(v));
   return op(v, partner<1>(v));
 }
@@ -546,9 +553,9 @@ FI_DEV RowSum join_sums(const ChunkSum* sums, int chunks, int lanes) {
 //
 // A thread reads its first kAhead keys at once, before sums() joins the rows'
 // sums: a join is one workgroup's chain of waits. The bound comes from groups of
-// those as a chunk's does. Further places are read in turn until one of all lists
-// holds nothing that reaches it. Where more reach it
-// than LDS holds (equal ones), the lists are merged, a choice a round.
+// those as a chunk's does. Further places are read in turn while the last one read
+// of some list reaches it. Where more reach it than LDS holds (equal ones), the
+// lists are merged, a choice a round.
 constexpr int kAhead = 8;
 constexpr int kLastBit = 8;  // of the bound: fifteen bits of mantissa
 template <int WAVES, class Key, class Sums, class Of, class Near, class Put>
@@ -634,18 +641,26 @@ FI_DEV void first_choices(const int lists, const int each, const int k,
     }
   }
   bound = larger(bound, 1u);
-  const auto take = [&](int step) {
+  // as many rounds as hold a place of all lists make a step
+  const int rounds = (lists + kAhead * T - 1) / (kAhead * T);
+  const auto take = [&](int round) {
+    const int step = round / rounds;
+    // a key's next one of its list is another step's from here on
+    const int beyond = (step + 1) * rounds * kAhead * T - lists;
     u64 reach[kAhead];
     int count = 0, at = 0;
+    bool more = false;
 #pragma unroll
     for (int n = 0; n < kAhead; ++n) {
       reach[n] = __ballot(of_got[n] >= bound);
       count += __popcll(reach[n]);
+      more |= of_got[n] >= bound && (round * kAhead + n) * T + tid >= beyond;
     }
     if (!count) return;
+    more = __ballot(more);
     if (lane == 0) {
       at = atomicAdd(&s_count, count);
-      s_reached[step % 2] = step + 1;
+      if (more) s_reached[step % 2] = step + 1;
       if (at + count > kTaken) s_full[step % 2] = step + 1;
     }
     at = __builtin_amdgcn_readfirstlane(at);
@@ -661,8 +676,6 @@ FI_DEV void first_choices(const int lists, const int each, const int k,
     }
   };
   take(0);
-  // as many rounds as hold a place of all lists make a step
-  const int rounds = (lists + kAhead * T - 1) / (kAhead * T);
   for (int n = 1; n * kAhead * T < N; ++n) {
     const int step = n / rounds;
     if (n % rounds == 0) {
@@ -675,7 +688,7 @@ FI_DEV void first_choices(const int lists, const int each, const int k,
     weigh(n * kAhead * T);
 #pragma unroll
     for (int q = 0; q < kAhead; ++q) of_got[q] = order(got[q].score);
-    take(step);
+    take(n);
   }
   __syncthreads();
   const int all = s_count;
