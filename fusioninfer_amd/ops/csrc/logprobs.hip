@@ -354,7 +354,7 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
   if (k) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (!__ballot(piece[i] >= bound)) continue;
+      if (held > kHeld || !__ballot(piece[i] >= bound)) continue;
       apart(raw[i]);
 #pragma unroll
       for (int e = 0; e < L; ++e) {
@@ -396,6 +396,7 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
       int count = 0;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
+        if (!__ballot(piece[i] > v)) continue;
         apart(raw[i]);
 #pragma unroll
         for (int e = 0; e < L; ++e) count += __popcll(__ballot(x[e] > v));
@@ -428,6 +429,9 @@ __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
     held = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      const bool wanted = equal < k - larger_ones ? piece[i] >= bound
+                                                  : piece[i] > bound;
+      if (!__ballot(wanted)) continue;
       apart(raw[i]);
       u64 same[L];
       int rank = equal;
