@@ -615,7 +615,11 @@ FI_DEV void first_choices(const int lists, const int each, const int k,
     top = larger(top, tops[w]);
   }
   const u64 best = over_wave(top, larger<u64>);
-  const auto order = [&](u64 score) { return score ? near(score, best) : 0; };
+  // where the first keys are all of dead rows there is nothing to be near to:
+  // whatever comes later reaches the bound
+  const auto order = [&](u64 score) -> u32 {
+    return !score ? 0 : best ? near(score, best) : 1;
+  };
   u32 of_got[kAhead], bound = 0;
 #pragma unroll
   for (int n = 0; n < kAhead; ++n) of_got[n] = order(got[n].score);

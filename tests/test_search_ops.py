@@ -465,3 +465,33 @@ def test_same_again():
     for _ in range(5):
         assert all(torch.equal(a, b)
                    for a, b in zip(first, ops.beam_select(x, c, 16)))
+
+
+# ------------------------------------------------- joins of many lists
+
+def alone_at(x, c, k, first):
+    """beams64 of the one search whose beams before `first` have no
+    continuation."""
+    s, p, t = beams64(x[first:], c[:, first:], k)
+    return s, np.where(p < 0, p, p + first), t
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["random", "steps"])
+@pytest.mark.parametrize("k", [1, 16, 100, 256])
+def test_last_beams_alone_go_on(dtype, kind, k):
+    """256 beams of ten chunks each: those whose first choices a join reads
+    first, 204 or more, have ended or no distribution."""
+    V = 9 * 32768 // dtype.itemsize + 1
+    x = rows_of(kind, 256, V, dtype, "cuda")
+    c = scores_of(1, 256)
+    c[0, :100] = -INF
+    x[100:180, 5] = float("nan")
+    x[180:230] = -INF
+    c[0, 230:253] = -INF
+    got = ops.beam_select(x, c.cuda(), k)
+    s, p, t = alone_at(x, c, k, 253)
+    assert np.array_equal(got.parents.cpu().numpy(), p)
+    assert np.array_equal(got.tokens.cpu().numpy(), t)
+    near(got.scores, s, V)
