@@ -547,7 +547,9 @@ FI_DEV RowSum join_sums(const ChunkSum* sums, int chunks, int lanes) {
   for (int c = at + kWaveSize; c < chunks; c += kWaveSize)
     s += sums[c].s * power(sums[c].m - from);
   s = over_lanes(s, lanes, [](double a, double b) { return a + b; });
-  return {log(s), m};
+  // one term is exp(0), but the instruction rounds it in two factors: below 1
+  // it would leave a log-probability above 0
+  return {s > 0.0 && s < 1.0 ? 0.0 : log(s), m};
 }
 
 // The first k of the choices that `lists` lists hold, `each` of them in order:

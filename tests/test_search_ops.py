@@ -495,3 +495,26 @@ def test_last_beams_alone_go_on(dtype, kind, k):
     assert np.array_equal(got.parents.cpu().numpy(), p)
     assert np.array_equal(got.tokens.cpu().numpy(), t)
     near(got.scores, s, V)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [2, 9, 20000])
+def test_no_probability_above_one(device, dtype, V):
+    """Rows that all but one token are masked in, whatever its logit is: the
+    sum is that token's term, and nothing rounds its log-probability above 0
+    or a score above its beam's."""
+    R = 2000 if V < 1000 else 64
+    g = torch.Generator().manual_seed(V)
+    at = torch.arange(R) * 7919 % V
+    x = torch.full((R, V), -INF)
+    x[torch.arange(R), at] = torch.randn(R, generator=g) * 30
+    x = x.to(dtype).to(device)
+    top = ops.top_logprobs(x, 1, at.to(device))
+    assert torch.equal(top.ids.view(-1).long().cpu(), at)
+    for lp in (top.logprobs.view(-1), top.token_logprobs):
+        assert (lp <= 0).all() and (lp >= -away(1)).all()
+    c = scores_of(R // 2, 2).to(device)
+    best = ops.beam_select(x, c, 2)
+    of = torch.gather(c, 1, best.parents.long())
+    assert (best.scores <= of).all()
