@@ -751,11 +751,11 @@ def copy_blocks_(tensors, src, dst, tokens=None) -> None:
     in one launch (one for each hundred tensors).
 
     tensors: contiguous tensors of any types and shapes on one device, their
-    first dimension the blocks of a paged cache or the slots of a state. src,
-    dst: int32 [pairs] on that device. tokens (int32 [pairs]): of paged
-    tensors [blocks, heads, block_size, width] only the first tokens[i] rows
-    of every head are copied, the others stay as they are; below 0 counts as
-    0, above block_size as block_size.
+    first dimension the blocks of a paged cache or the slots of a state, each
+    smaller than 2 GiB on a GPU. src, dst: int32 [pairs] on that device.
+    tokens (int32 [pairs]): of paged tensors [blocks, heads, block_size,
+    width] only the first tokens[i] rows of every head are copied, the others
+    stay as they are; below 0 counts as 0, above block_size as block_size.
 
     A pair with an id outside a tensor's blocks (-1, say, as padding) copies
     nothing there. A block may be the source of many pairs; one that is a

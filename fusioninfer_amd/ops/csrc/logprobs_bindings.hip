@@ -153,42 +153,33 @@ void copy_blocks(const std::vector<at::Tensor>& tensors,
   c10::optional<at::Tensor> tokens;
   if (token_counts) tokens = ids(*token_counts);
   CHECK_THAT(pairs < (1ll << 31), "too many pairs");
+  // every tensor is checked before the first launch
+  std::vector<fi::BlockTensors> tables;
+  int64_t count = 0;
   int block_size = -1;
   for (const auto& t : tensors) {
     CHECK_THAT(t.dim() >= 1 && t.is_contiguous(),
                "tensors of blocks are contiguous");
     CHECK_THAT(t.device() == src.device(),
                "tensors and ids are on one device");
-    if (!tokens) continue;
-    CHECK_THAT(t.dim() == 4 && t.size(2) < (1ll << 31) &&
-                   (block_size < 0 || t.size(2) == block_size),
-               "tokens go with paged tensors [blocks, heads, block_size, "
-               "width] of one block_size");
-    block_size = static_cast<int>(t.size(2));
-  }
-  if (pairs == 0) return;
-  const Guard guard(src.device());
-  fi::BlockTensors table;
-  int count = 0;
-  const auto flush = [&] {
-    if (count == 0) return;
-    fi::launch_copy_blocks(table, count, src.data_ptr<int>(),
-                           dst.data_ptr<int>(),
-                           tokens ? tokens->data_ptr<int>() : nullptr, pairs,
-                           block_size, current_stream());
-    check_launch();
-    count = 0;
-  };
-  for (const auto& t : tensors) {
+    if (tokens) {
+      CHECK_THAT(t.dim() == 4 && t.size(2) < (1ll << 31) &&
+                     (block_size < 0 || t.size(2) == block_size),
+                 "tokens go with paged tensors [blocks, heads, block_size, "
+                 "width] of one block_size");
+      block_size = static_cast<int>(t.size(2));
+    }
     if (t.numel() == 0) continue;
     const int64_t block = t.numel() / t.size(0) * t.element_size();
     const int64_t heads = tokens ? t.size(1) : 1;
     const int64_t token = tokens ? t.size(3) * t.element_size() : block;
     CHECK_THAT(block < (1ll << 31) && t.size(0) < (1ll << 31),
-                "a block must be smaller than 2 GiB");
+               "a block must be smaller than 2 GiB");
     const auto bits =
         reinterpret_cast<uintptr_t>(t.data_ptr()) | block | token;
-    fi::BlockTensor& e = table.t[count++];
+    const int64_t at = count++ % fi::kBlockTensors;
+    if (at == 0) tables.emplace_back();
+    fi::BlockTensor& e = tables.back().t[at];
     e.data = static_cast<char*>(t.data_ptr());
     e.head_bytes = static_cast<fi::u32>(block / heads);
     e.token_bytes = static_cast<fi::u32>(token);
@@ -197,9 +188,17 @@ void copy_blocks(const std::vector<at::Tensor>& tensors,
                                 fi::kSliceBytes);
     e.blocks = static_cast<int>(t.size(0));
     e.unit = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
-    if (count == fi::kBlockTensors) flush();
   }
-  flush();
+  if (pairs == 0) return;
+  const Guard guard(src.device());
+  for (const auto& table : tables) {
+    fi::launch_copy_blocks(table, std::min<int64_t>(count, fi::kBlockTensors),
+                           src.data_ptr<int>(), dst.data_ptr<int>(),
+                           tokens ? tokens->data_ptr<int>() : nullptr, pairs,
+                           block_size, current_stream());
+    check_launch();
+    count -= fi::kBlockTensors;
+  }
 }
 
 }  // namespace

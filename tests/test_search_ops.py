@@ -518,3 +518,14 @@ def test_no_probability_above_one(device, dtype, V):
     best = ops.beam_select(x, c, 2)
     of = torch.gather(c, 1, best.parents.long())
     assert (best.scores <= of).all()
+
+
+@pytest.mark.gpu
+def test_refused_copies_copy_nothing():
+    """A block of 2 GiB behind more tensors than one launch takes."""
+    ts = [bits((2, 4), torch.float32, "cuda", i) for i in range(120)]
+    old = [t.clone() for t in ts]
+    ts.append(torch.empty(1, 1 << 31, dtype=torch.uint8, device="cuda"))
+    with pytest.raises(ValueError):
+        ops.copy_blocks_(ts, ints([0], "cuda"), ints([1], "cuda"))
+    assert all(same_bytes(a, b) for a, b in zip(ts, old))
