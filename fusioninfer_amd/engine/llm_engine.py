@@ -1209,9 +1209,12 @@ class LLMEngine:
         seats = self.cfg.scheduler.max_num_seqs
         if self.state_manager is not None:
             seats = min(seats, self.state_manager.num_free())
-        if not 1 <= beam_width <= min(seats, ops.MOST_BEAMS):
+        # as many beams as one choice over their vocabulary takes
+        most = min(seats, ops.MOST_BEAMS,
+                   ops.MOST_CHUNKS // -(-self.cfg.model.vocab_size // 8192))
+        if not 1 <= beam_width <= most:
             raise ValueError(f"beam_width {beam_width} is not from 1 to "
-                             f"{min(seats, ops.MOST_BEAMS)}")
+                             f"{most}")
         if max_tokens < 1:
             raise ValueError("max_tokens is at least 1")
         for p in prompts:

@@ -212,6 +212,16 @@ def test_refusals():
     nothing_held(eng)
 
 
+def test_refuses_more_beams_than_a_choice_takes(monkeypatch):
+    """Before the first step: 256 beams of a vocabulary beyond 163840, say."""
+    eng = make_engine()
+    monkeypatch.setattr(ops, "MOST_CHUNKS", 3)
+    with pytest.raises(ValueError):
+        eng.beam_search([[1, 2, 3]], 4)
+    assert eng.num_prefilled_tokens == 0
+    assert len(eng.beam_search([[1, 2, 3]], 3, max_tokens=2)[0]) == 3
+
+
 def test_fork_of_blocks():
     bm = BlockManager(8, 4)
     a = Sequence("a", [1] * 10, SamplingParams())
