@@ -1196,8 +1196,9 @@ class LLMEngine:
         log-probability over length ** length_penalty. ``stop_token_ids`` end
         a hypothesis, as does max_model_len; without any, all have
         ``max_tokens`` tokens. Searches run side by side as far as
-        max_num_seqs holds their beams, beside requests that are served, and
-        raise InsufficientBlocksError where the cache cannot hold them. A step
+        max_num_seqs holds their beams, beside requests that are served; where
+        the cache cannot hold them they start again, half as many at once, and
+        one that it cannot hold by itself raises InsufficientBlocksError. A step
         looks at the ops.MOST_CHOICES best continuations of a search at most:
         where so many of them end that fewer than ``beam_width`` are left, it
         goes on with those."""
@@ -1223,9 +1224,15 @@ class LLMEngine:
                                  f"within max_model_len {limit}")
         out = []
         at_once = seats // beam_width
-        for i in range(0, len(prompts), at_once):
-            out += BeamSearcher(self, beam_width, max_tokens, stop_token_ids,
-                                length_penalty).run(prompts[i: i + at_once])
+        while len(out) < len(prompts):
+            group = prompts[len(out): len(out) + at_once]
+            try:
+                out += BeamSearcher(self, beam_width, max_tokens,
+                                    stop_token_ids, length_penalty).run(group)
+            except InsufficientBlocksError:
+                if len(group) == 1:
+                    raise
+                at_once = (len(group) + 1) // 2
         return out
 
     def generate(

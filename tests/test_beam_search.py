@@ -173,6 +173,22 @@ def test_blocks_run_out():
     nothing_held(eng)
 
 
+def test_fewer_searches_at_once_where_blocks_run_out(monkeypatch):
+    """Seats for eight searches, blocks for two of them."""
+    from fusioninfer_amd.engine import beam_search as module
+
+    tried, run = [], module.BeamSearcher.run
+    monkeypatch.setattr(module.BeamSearcher, "run", lambda self, prompts: (
+        tried.append(len(prompts)), run(self, prompts))[1])
+    eng = make_engine(blocks=8)
+    prompts = [[(9 * i + n) % 1024 for i in range(30)] for n in range(5)]
+    got = eng.beam_search(prompts, 2, max_tokens=2)
+    assert tried[0] == 5 and sum(tried[-3:]) == 5
+    for g, p in zip(got, prompts):
+        agree(g, plain_search(eng, p, 2, 2))
+    nothing_held(eng)
+
+
 def test_served_requests_stay_as_they_are():
     """A search between the steps of requests that are served."""
     prompts = [[9, 8, 7] * 7, [4] * 30]
