@@ -8,6 +8,7 @@ TP via symmetric SPMD stepping, see distributed/parallel_state.py).
 from __future__ import annotations
 
 import itertools
+import math
 import os
 import time
 from typing import Dict, List, Optional
@@ -1218,6 +1219,11 @@ class LLMEngine:
                              f"{most}")
         if max_tokens < 1:
             raise ValueError("max_tokens is at least 1")
+        # also refuses what is no number
+        longest = max(2, min(max_tokens, limit))
+        if not abs(length_penalty) * math.log(longest) < 500:
+            raise ValueError(f"length_penalty {length_penalty} leaves no "
+                             "scores to compare")
         for p in prompts:
             if not 1 <= len(p) < limit:
                 raise ValueError(f"prompt length {len(p)} leaves no room "

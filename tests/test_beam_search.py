@@ -238,6 +238,19 @@ def test_refuses_more_beams_than_a_choice_takes(monkeypatch):
     assert len(eng.beam_search([[1, 2, 3]], 3, max_tokens=2)[0]) == 3
 
 
+@pytest.mark.parametrize("penalty", [float("nan"), float("inf"), 400.0,
+                                     -400.0])
+def test_refuses_length_penalties_out_of_range(penalty):
+    """Lengths to their power would be infinite, or 0."""
+    eng = make_engine()
+    with pytest.raises(ValueError):
+        eng.beam_search([[1, 2, 3]], 2, max_tokens=8, length_penalty=penalty)
+    assert eng.num_prefilled_tokens == 0
+    for p in (50.0, -50.0):
+        got, = eng.beam_search([[1, 2, 3]], 2, max_tokens=8, length_penalty=p)
+        assert all(math.isfinite(h.score) for h in got)
+
+
 def test_fork_of_blocks():
     bm = BlockManager(8, 4)
     a = Sequence("a", [1] * 10, SamplingParams())
