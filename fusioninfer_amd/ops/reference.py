@@ -438,12 +438,23 @@ def _first_of(values: torch.Tensor, k: int) -> torch.Tensor:
 def top_logprobs(logits, k: int, token_ids=None):
     """fp32 log_softmax; a row without a distribution is NaN throughout and
     lists its first k tokens."""
-    lp = torch.log_softmax(logits.float(), dim=-1)
+    x = logits.float()
+    lp = torch.log_softmax(x, dim=-1)
     R, V = lp.shape
     ids = torch.arange(k, dtype=torch.int32).repeat(R, 1)
-    for r in range(R):
-        if k and not torch.isnan(lp[r]).any():
-            ids[r] = _first_of(logits[r].float(), k)
+    if k and R:
+        some = ~torch.isnan(lp[:, 0])
+        # all rows at once; alone only those whose k-th is one of equal ones
+        first = x.topk(min(k + 1, V), dim=1)
+        at = first.indices[:, :k].sort(dim=1).values
+        order = torch.gather(x, 1, at).sort(dim=1, descending=True,
+                                            stable=True).indices
+        at = torch.gather(at, 1, order).int()
+        ids = torch.where(some.view(-1, 1), at, ids)
+        if k < V:
+            among = some & (first.values[:, k - 1] == first.values[:, k])
+            for r in torch.nonzero(among).view(-1).tolist():
+                ids[r] = _first_of(x[r], k)
     top = torch.gather(lp, 1, ids.long())
     if token_ids is None:
         return top, ids, None
