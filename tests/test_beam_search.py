@@ -349,3 +349,41 @@ def test_gpu_logprobs_of_requests():
     of, top = out.logprobs[0]
     assert out.output_token_ids[0] in top and len(top) == 4
     assert top[out.output_token_ids[0]] == of == max(top.values())
+
+
+@pytest.mark.parametrize("device", [
+    "cpu", pytest.param("cuda:0", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("batch", [1, 5])
+def test_logprobs_are_those_of_the_logits(device, batch, monkeypatch):
+    """What requests are given against torch's log-softmax, in 64 bits, of the
+    same logits; decode steps of one row, too."""
+    from test_search_ops import HALF, away
+
+    seen, entries_of = [], LLMEngine._logprob_entries
+
+    def entries(self, logits, ks, ids):
+        before = logits.double().cpu()
+        got = entries_of(self, logits, ks, ids)
+        seen.append((before, list(ks), list(ids), got))
+        return got
+
+    monkeypatch.setattr(LLMEngine, "_logprob_entries", entries)
+    eng = make_engine(device, layers=2, blocks=256, **(
+        {} if device == "cpu" else {"model": "Qwen3-0.6B"}))
+    prompts = [[(17 * i + n) % 1000 for i in range(20 + n)]
+               for n in range(batch)]
+    eng.generate(prompts, SamplingParams(max_tokens=3, logprobs=7,
+                                         prompt_logprobs=20))
+    assert min(len(ks) for _, ks, _, _ in seen) == batch \
+        and max(len(ks) for _, ks, _, _ in seen) >= 19
+    for logits, ks, ids, got in seen:
+        lp = torch.log_softmax(logits, 1)
+        off = away(lp.shape[1])
+        for row, k, t, (of, top) in zip(lp, ks, ids, got):
+            assert abs(of - row[t].item()) <= off - HALF * row[t].item()
+            want = row.topk(k).values
+            assert len(top) == k
+            for v, (i, w) in zip(want.tolist(), top.items()):
+                # the i-th, and its own token's
+                assert abs(w - v) <= off - HALF * v
+                assert abs(w - row[i].item()) <= off - HALF * v

@@ -49,3 +49,7 @@ def test_no_flat_accesses_beside_counted_waits(source, tmp_path):
     text = asm.read_text()
     assert re.search(r"s_waitcnt vmcnt\([1-9]", text)
     assert not re.findall(r"\bflat_(?:load|store|atomic)\w*", text)
+
+
+def test_no_kernel_of_log_probabilities_spills():
+    test_no_kernel_spills("logprobs.hip", "")

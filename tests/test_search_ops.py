@@ -529,3 +529,85 @@ def test_refused_copies_copy_nothing():
     with pytest.raises(ValueError):
         ops.copy_blocks_(ts, ints([0], "cuda"), ints([1], "cuda"))
     assert all(same_bytes(a, b) for a, b in zip(ts, old))
+
+
+def close(got, want, V):
+    """As near(), for logits below 2^15 on a GPU. A term exp(t): the exponent
+    t log2(e) is rounded once, |t| half steps, and the constant off by 0.23 of
+    one, with |t| at most ln V on average; the exponential by a step. Three
+    additions in 32 bits, then all in 64. A chunk's sum is scaled twice, each
+    time by an exponential (a step) of an exponent below 0.5 (half a one)."""
+    off = (1.23 * math.log(max(V, 2)) + 2 + 3 + 2 * 2.5) * HALF
+    got = got.double().cpu().numpy()
+    assert np.array_equal(np.isfinite(got), np.isfinite(want))
+    some = np.isfinite(want)
+    assert np.all(np.abs(got[some] - want[some])
+                  <= off + HALF * np.abs(want[some]))
+
+
+def first64(x, k):
+    """Of rows on the GPU, without NaN: logits, log-probabilities and tokens of
+    the k first, equal ones by token."""
+    at = x.float().sort(dim=1, descending=True, stable=True).indices[:, :k]
+    lp = torch.cat([torch.log_softmax(r.double(), 1) for r in x.split(32)])
+    return [torch.gather(t, 1, at).double().cpu().numpy()
+            for t in (x.float(), lp)] + [at.cpu().numpy()]
+
+
+def one_search64(x, c, k):
+    """beams64 of one search, by its beams' first tokens."""
+    logit, lp, token = first64(x, k)
+    beam = np.arange(len(x))[:, None].repeat(k, 1)
+    s = c.double().numpy().reshape(-1, 1) + lp
+    first = np.lexsort([a.reshape(-1) for a in (token, -logit, beam, -s)])[:k]
+    return [a.reshape(-1)[first] for a in (s, beam, token)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("R,V,k", [
+    (1, 151936, 20), (1, 151936, 0), (1, 151936, 256), (3, 1_000_003, 5),
+    (2, 2_500_000, 64)])
+@pytest.mark.parametrize("kind", ["random", "rising", "equal", "clustered"])
+def test_rows_of_many_chunks(dtype, R, V, k, kind):
+    """Up to 306 chunks a row, more than a wave has lanes; "rising": the last
+    ones hold most of the sum and all choices."""
+    x = rows_of(kind, R, V, dtype, "cuda", pad=1)
+    given = torch.arange(R) * 7919 + V - 1 - R * 7919
+    got = ops.top_logprobs(x, k, given.cuda())
+    _, lp, token = first64(x, max(k, 1))
+    assert np.array_equal(got.ids.cpu().numpy(), token[:, :k])
+    close(got.logprobs, lp[:, :k], V)
+    lp = torch.log_softmax(x.double(), 1).cpu()
+    close(got.token_logprobs, lp[torch.arange(R), given].numpy(), V)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["random", "steps", "equal", "plateau"])
+@pytest.mark.parametrize("B,V,k", [
+    (64, 41_000, 64), (64, 41_000, 256),        # 384 or 192 lists
+    (256, 151_936, 16), (256, 151_936, 256)])   # 4864 or 2560
+def test_one_search_of_many_lists(dtype, kind, B, V, k):
+    """More lists than a join has threads, and than it reads at once."""
+    x = rows_of(kind, B, V, dtype, "cuda")
+    c = scores_of(1, B, kind)
+    got = ops.beam_select(x, c.cuda(), k)
+    s, b, t = one_search64(x, c, k)
+    assert np.array_equal(got.parents.cpu().numpy()[0], b)
+    assert np.array_equal(got.tokens.cpu().numpy()[0], t)
+    close(got.scores[0], s, V)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["random", "steps", "equal", "plateau",
+                                  "clustered", "masked"])
+@pytest.mark.parametrize("k", [33, 50, 64])
+def test_many_choices_by_one_wave(dtype, kind, k):
+    """Few chunks a row and more choices than half a wave's lanes."""
+    x = rows_of(kind, 40, 50_021, dtype, "cuda", pad=2, start=1)
+    got = ops.top_logprobs(x, k)
+    _, lp, token = first64(x, k)
+    assert np.array_equal(got.ids.cpu().numpy(), token)
+    close(got.logprobs, lp, x.shape[1])
