@@ -12,6 +12,10 @@ a step needs no more blocks than its beams hold.
 A continuation that ends with a stop token is a finished hypothesis if it ranks
 before the last beam kept; hypotheses are ordered by cumulative log-probability
 over length ** length_penalty.
+
+A cumulative log-probability is rounded to fp32 at every step, as
+``beam_select`` takes and gives it: at -1000 by up to 3e-5 a step. Beams nearer
+to one another than that may change places, or be equal and go by beam.
 """
 
 from __future__ import annotations

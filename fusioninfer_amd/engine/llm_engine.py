@@ -890,9 +890,9 @@ class LLMEngine:
         logits_rows covering every prompt position of requesting
         sequences; fill seq.prompt_logprobs (index 0 and prefix-cached
         positions are None) and return the standard sampling-row subset
-        in the engine's expected order. Where a log-softmax has to be formed,
-        rows are taken in slices, so that a full 8k-token admission never
-        materializes a [T, V] fp32."""
+        in the engine's expected order. logits_f are all rows in fp32; of a
+        log-softmax, where one has to be formed, there are never more than
+        256 rows."""
         rows = payload["logits_rows"]
         pos_of = {r: i for i, r in enumerate(rows)}
         cu = payload["cu"]

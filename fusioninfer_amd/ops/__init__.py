@@ -1235,7 +1235,8 @@ def top_logprobs(logits: torch.Tensor, k: int,
     ordered by logit, equal ones by token, those at -inf last. A row without a
     distribution (a NaN or +inf in it, or -inf throughout) is NaN, its tokens
     0 to k-1. A given token outside [0, V) has -inf. k: 0 to V, at most
-    MOST_CHOICES; V: up to some 40 million."""
+    MOST_CHOICES; V: up to some 40 million, and on a GPU no more than 17
+    billion logits and 16 million rows in a call. None is above 0."""
     if logits.is_cuda:
         _require_native()
         return TopLogprobs(*_C.top_logprobs(logits, k, token_ids))
@@ -1269,7 +1270,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor,
     begun) or whose row has no distribution (a NaN or +inf in it). Places
     without a continuation hold score -inf, beam -1 and token -1.
 
-    B: up to MOST_BEAMS, and B times V up to some 40 million. k: 1 to
+    B: up to MOST_BEAMS, and B times V up to some 40 million (B times V /
+    8192, rounded up, at most MOST_CHUNKS). k: 1 to
     MOST_CHOICES; twice the number of beams leaves enough of them where up to
     one continuation of each beam ends it."""
     if logits.is_cuda:

@@ -147,11 +147,13 @@ template void launch_kv_block_copy<false>(u16*, u16*, u16*, const int*, int,
 // that are filled. A wave copies one slice of one head of one block. Pairs
 // with an id outside the tensor are passed over.
 //
-// What is written is not read again by this launch: stored past the caches it
-// takes 36 us for 239 MB of states and 116 us for 805 MB of whole e4m3 pages,
-// 42 and 128 through them; loads past the caches lose (40 and 140), as beams
-// that go on from the same page read it again. 320 pages of 72 tensors, half
-// full, 802 MB: 154 us, 5.2 TB/s, where a copy of 2 GiB reaches 5.0.
+// What is written is not read again by this launch: stored past the caches 48
+// slots of states take 36.5 us and 512 whole e4m3 pages of 96 tensors 116, 41 and
+// 127 through them; loads past the caches lose (40 and 139), as beams that go on
+// from the same page read it again. Of separate blocks a copy of 2 GiB reads and
+// writes 5.1 TB/s (torch's copy 4.8 to 5.0); 320 pages of 72 tensors, half full,
+// some of them the source of several copies, take 150 to 157 us, 4.4 to 4.6 TB/s
+// of what differs.
 __global__ __launch_bounds__(256) void copy_blocks_kernel(
     const BlockTensors tensors, const int* __restrict__ src,
     const int* __restrict__ dst, const int* __restrict__ tokens,

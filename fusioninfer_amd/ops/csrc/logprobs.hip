@@ -30,13 +30,18 @@ using u64 = unsigned long long;
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWaveSize;
+// 1.3e-8 too small, relatively: a term exp(-t) comes out by 1.3e-8 t too large,
+// and ln S by as much with the terms' mean t, at most ln V (top 1 of 1531 rows is
+// off by 5.7e-8 of itself, of which rounding to fp32 is 2.6e-8). The constant's
+// rest would cost an instruction a logit.
 constexpr float kLog2e = 1.44269504f;
 
 FI_DEV float logit_of(const float* p) { return *p; }
 FI_DEV float logit_of(const u16* p) { return bf16_to_f32(*p); }
 
-// 16 bytes of logits from anywhere, past the caches: 2048 rows 94 us a call, 106
-// through them
+// 16 bytes of logits from anywhere, past the caches: 2048 rows 95 us a call, 107
+// through them, 1531 rows 77 and 86; 80 rows of 32000, which the caches still hold
+// from the call before, 13.1 and 11.7
 FI_DEV u32x4 read_once(const void* p) {
   typedef u32x4 __attribute__((aligned(2))) Anywhere;
   return __builtin_nontemporal_load(static_cast<const Anywhere*>(p));
@@ -191,13 +196,14 @@ FI_DEV u32 reached_by(const u32 (&order)[N], int k) {
 // are counted from the row's first logit wherever it lies, so that
 // equal rows have equal sums; what the last group lacks counts as -inf.
 //
-// About six instructions a bf16 logit, one of them the exponential of four
-// times the cycles, are what memory leaves time for (2048 rows of 152064: 94 us
-// a call, 6.6 TB/s), so everything else is done per piece or per thread: sums go
-// on in 64 bits every piece (a sum that one term dominates keeps the others),
-// the bound is found from the threads' maxima, and the logits of a piece are
-// looked at only where its maximum reaches it. Finding 16 of each row costs a
-// fifth more than none (512 rows of 151936: 32.5 us and 27).
+// Without choices it takes 7.6 vector instructions a bf16 logit, one of them the
+// exponential of four times the cycles, about what memory leaves time for (2048
+// rows of 152064: 95 us a call, 6.5 TB/s), so everything else is done per piece
+// or per thread: sums go on in 64 bits every piece, after three additions in 32
+// bits of bf16 logits and two of fp32 (a sum that one term dominates keeps the
+// others), the bound is found from the threads' maxima, and the logits of a piece
+// are looked at only where its maximum reaches it. With 16 choices it is 11
+// instructions (512 rows of 151936: 31 to 32 us, 27 without).
 template <typename A, int NV>
 __global__ __launch_bounds__(kThreads) void logit_chunks_kernel(
     const A* __restrict__ logits, const int64_t stride, const int V,
@@ -772,8 +778,8 @@ FI_DEV void first_choices(const int lists, const int each, const int k,
 }
 
 // One workgroup per search: the k best of its beams' first tokens. Sixteen waves
-// are slower than four even where 32 beams hand on 16384 keys (29 and 27 us a
-// call).
+// are slower than four even where 32 beams hand on 16384 keys (32 to 33 us a call,
+// 24.5 with four), and for one search of 4 beams (12.3 and 10.6).
 __global__ __launch_bounds__(kThreads) void beam_join_kernel(
     const ChunkSum* __restrict__ sums, const u64* __restrict__ keys,
     const int chunks, const float* __restrict__ scores,
@@ -903,10 +909,12 @@ struct Cut {
 // Chunks as large as registers hold, 8 pieces a thread, leave the least to
 // join; halved until 64 workgroups share the call, as long as a chunk has four
 // times as many pieces as it gives keys (256 choices of one row 32 us, 142
-// without). With the joins of that step one search of 4 beams over 151936 tokens
-// took 12.3 us so, 14.1 by 256 to 2048 workgroups, which read faster but leave
-// twice as much to join; 64 searches of 8 beams 47 us, 49 with 4 pieces. Sixteen
-// pieces are no faster.
+// without). One search of 4 beams over 151936 tokens takes 10.6 us a call so, 11.4
+// to 11.7 by 256 and 2048 workgroups, which read faster but leave more to join, 2
+// searches of 32 beams 24.4, by 2048 workgroups 31.7. With 4 and 16 pieces at most
+// 64 searches of 8 beams take 45.5 and 42.3 us, 38.2 with 8; top tokens of 1531
+// rows 82, 79 and 77. Some small calls would gain by 4: 80 fp32 rows of 32000
+// 11.9 us for 13.1, 61 of 151936 14.4 for 15.1.
 Cut cut_of(int64_t R, int V, int k, int size) {
   const int lanes = 16 / size;
   const int pieces = (V + lanes - 1) / lanes;
