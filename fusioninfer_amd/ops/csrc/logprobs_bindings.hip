@@ -169,7 +169,7 @@ void copy_blocks(const std::vector<at::Tensor>& tensors,
                  "width] of one block_size");
       block_size = static_cast<int>(t.size(2));
     }
-    if (t.numel() == 0) continue;
+    if (pairs == 0 || t.numel() == 0) continue;
     const int64_t block = t.numel() / t.size(0) * t.element_size();
     const int64_t heads = tokens ? t.size(1) : 1;
     const int64_t token = tokens ? t.size(3) * t.element_size() : block;
@@ -189,7 +189,6 @@ void copy_blocks(const std::vector<at::Tensor>& tensors,
     e.blocks = static_cast<int>(t.size(0));
     e.unit = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
   }
-  if (pairs == 0) return;
   const Guard guard(src.device());
   for (const auto& table : tables) {
     fi::launch_copy_blocks(table, std::min<int64_t>(count, fi::kBlockTensors),

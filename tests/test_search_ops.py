@@ -529,6 +529,7 @@ def test_refused_copies_copy_nothing():
     with pytest.raises(ValueError):
         ops.copy_blocks_(ts, ints([0], "cuda"), ints([1], "cuda"))
     assert all(same_bytes(a, b) for a, b in zip(ts, old))
+    ops.copy_blocks_(ts, ints([], "cuda"), ints([], "cuda"))
 
 
 def close(got, want, V):
